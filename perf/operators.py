@@ -222,7 +222,7 @@ def _plain_logprobs(s):
     total = e.sum(-1, keepdim=True)
     at = s["targets"][:, None]
     logps = (x.gather(1, at) - top - total.log())[:, 0]
-    return x, e, total, (top + total.log())[:, 0], logps
+    return e, total, top, logps
 
 
 def _plain_dlogits(s, e, total, dlogps):
@@ -233,7 +233,7 @@ def _plain_dlogits(s, e, total, dlogps):
 
 def _plain_preference(s):
     c = s["case"]
-    _, e, total, _, logps = _plain_logprobs(s)
+    e, total, _, logps = _plain_logprobs(s)
     ratio = torch.where(s["mask"], logps.view(s["ref"].shape).double() - s["ref"], 0.0)
     r = ratio.sum(-1)
     if c["form"] == "sigmoid":
@@ -253,7 +253,7 @@ def _plain_preference(s):
 
 
 def _plain_policy(s):
-    _, e, total, _, logps = _plain_logprobs(s)
+    e, total, _, logps = _plain_logprobs(s)
     A, w = s["advantages"], s["weights"]
     ratio = (logps - s["old"]).exp()
     free, bound = -A * ratio, -A * ratio.clamp(0.8, 1.2)
@@ -292,16 +292,17 @@ def _own_loss(s):
     c = s["case"]
     V = c["vocab"]
     if c["op"] == "logprobs":
-        return dict(zip(("logps", "lse"), ops.token_logprobs(s["logits"], V, s["targets"])))
+        logps, stats = ops.token_logprobs(s["logits"], V, s["targets"])
+        return {"logps": logps, "stats": stats}
     if c["op"] == "policy":
         loss, logps, dlogits = ops.policy_loss_chunk(
             s["logits"], V, s["targets"], s["old"], s["advantages"], s["weights"], ref_logps=s["ref"], clip_low=0.2,
             clip_high=0.2, kl_coef=0.05)
         return {"loss": loss, "logps": logps, "dlogits": dlogits[:, :V]}
-    logps, lse = ops.token_logprobs(s["logits"], V, s["targets"])
+    logps, stats = ops.token_logprobs(s["logits"], V, s["targets"])
     loss, rewards, dlogps = ops.preference_loss(logps.view(s["ref"].shape), s["ref"], s["mask"], beta=0.1,
                                                 form=c["form"], grad_scale=1.0 / c["pairs"])
-    dlogits = ops.token_logprobs_bwd(s["logits"], V, s["targets"], lse, dlogps)
+    dlogits = ops.token_logprobs_bwd(s["logits"], V, s["targets"], stats, dlogps)
     return {"loss": loss, "rewards": rewards, "logps": logps, "dlogits": dlogits[:, :V]}
 
 
@@ -310,8 +311,8 @@ def run(state):
     if own:
         return (_own_heads if op.startswith("heads") else _own_dropout if op == "dropout" else _own_loss)(state)
     if op == "logprobs":
-        _, _, _, lse, logps = _plain_logprobs(state)
-        return {"logps": logps, "lse": lse}
+        _, total, top, logps = _plain_logprobs(state)
+        return {"logps": logps, "stats": torch.cat([top, total], 1)}
     return {"heads_fwd": _plain_heads, "heads_bwd": _plain_heads, "dropout": _plain_dropout,
             "preference": _plain_preference, "policy": _plain_policy}[op](state)
 
@@ -327,7 +328,7 @@ def work(case):
     rows = 2 * case["pairs"] * case["seq"] if op == "preference" else case["rows"]
     n = rows * case["vocab"]
     if op == "logprobs":
-        return {"bytes": n * e + 16 * rows, "flops": 4 * n}
+        return {"bytes": n * e + 20 * rows, "flops": 4 * n}
     return {"bytes": 2 * n * e + (28 if op == "policy" else 17) * rows, "flops": 7 * n}
 
 
@@ -392,7 +393,8 @@ def _exact_loss(s):
         lse[a:a + block] = torch.logsumexp(x, -1)
         logps[a:a + block] = x[torch.arange(len(x)), s["targets"][a:a + block]] - lse[a:a + block]
     if op == "logprobs":
-        return {"logps": logps, "lse": lse}
+        top = s["logits"][:, :V].amax(1).double()
+        return {"logps": logps, "stats": torch.stack([top, torch.exp(lse - top)], 1)}
     if op == "policy":
         A, w, k = s["advantages"].double(), s["weights"].double(), 0.05
         ratio, back = torch.exp(logps - s["old"].double()), torch.exp(s["ref"].double() - logps)
