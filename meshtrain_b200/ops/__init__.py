@@ -10,6 +10,9 @@ backward (no autograd inside).  Dispatch rule, per call:
   restatement of the same math.  That path is the numerics oracle for the
   kernels, the fp32 parity path, and what runs on CPU-only hosts.
 
+``qk_norm_rope``, ``dropout``, ``token_logprobs``, ``policy_loss_chunk`` and their
+backwards have kernels for bf16, fp16 and fp32 alike.
+
 The reference runs all of these as stock PyTorch ops (reference
 models/tiny_transformer.py:19-59, runtime/stage.py:28-36); here they are the
 replacement kernels' entry points.
@@ -35,7 +38,7 @@ EPI_BF16, EPI_GELU, EPI_RESID, EPI_DGELU, EPI_F32, EPI_SWIGLU = range(6)
 # Kernel launches issued through this module since import (each binding call
 # launches one kernel; the attention bindings report their own count).
 LAUNCHES = 0
-_MULTI_LAUNCH = {"attention_fwd": 1, "attention_bwd": 3}
+_MULTI_LAUNCH = {"attention_fwd": 1, "attention_bwd": 3, "qk_norm_rope_bwd": 2}
 _NO_LAUNCH = {"read_status"}
 
 
@@ -127,6 +130,34 @@ def _custom(*tensors: torch.Tensor) -> bool:
     return True
 
 
+_KERNEL_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _custom_float(t: torch.Tensor) -> bool:
+    """``_custom`` for the operators whose kernels also take fp16 and fp32."""
+    if not (t.is_cuda and _BACKEND == "custom" and t.dtype in _KERNEL_DTYPES):
+        return False
+    extension()
+    return True
+
+
+def _acc(t: torch.Tensor) -> torch.dtype:
+    """Type the plain restatements compute in."""
+    return torch.float64 if t.dtype == torch.float64 else torch.float32
+
+
+def _require(ok: bool, message: str) -> None:
+    if not ok:
+        raise ValueError(message)
+
+
+def _vector(t: torch.Tensor, n: int, like: torch.Tensor, dtype: torch.dtype, name: str) -> torch.Tensor:
+    """``t`` as a contiguous vector of ``n`` values of ``dtype`` on ``like``'s device."""
+    _require(t.numel() == n and t.dtype == dtype and t.device == like.device,
+             f"{name} must have {n} values of {dtype} on {like.device}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
+    return t.reshape(-1).contiguous()
+
+
 def _mat(x: torch.Tensor) -> torch.Tensor:
     """2-D row-major view suitable for TMA: unit column stride, row stride a
     multiple of 8 elements (16 bytes), 16-byte aligned base.  Rows whose width
@@ -140,6 +171,12 @@ def _mat(x: torch.Tensor) -> torch.Tensor:
     buf = torch.empty(rows, ld, dtype=x2.dtype, device=x2.device)
     buf[:, :cols] = x2
     return buf[:, :cols]
+
+
+def _aligned(x: torch.Tensor) -> torch.Tensor:
+    """``x`` contiguous and starting on a 16-byte boundary (a copy where it is not)."""
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
 # ----------------------------------------------------------------------------- linear
@@ -432,6 +469,181 @@ def rope_(qk: torch.Tensor, seq_len: int, heads: int, head_dim: int, theta: floa
     qk[:, : heads * head_dim] = torch.cat([o1, o2], -1).reshape(T, heads * head_dim).to(qk.dtype)
 
 
+def _check_heads(name, qkv, q_gain, k_gain, seq_len, heads, kv_heads, head_dim, theta, eps) -> int:
+    _require(qkv.dim() == 2 and heads >= 0 and kv_heads >= 0 and heads + kv_heads >= 1 and head_dim >= 2
+             and head_dim % 2 == 0 and qkv.shape[1] >= (heads + kv_heads) * head_dim,
+             f"{name}: qkv must be [rows, >= (heads + kv_heads) * head_dim] with an even head_dim")
+    _require(seq_len >= 1 and theta > 0 and eps >= 0, f"{name}: needs seq_len >= 1, theta > 0 and eps >= 0")
+    for g, what in ((q_gain, "q_gain"), (k_gain, "k_gain")):
+        _require(tuple(g.shape) == (head_dim,) and g.dtype == qkv.dtype and g.device == qkv.device,
+                 f"{name}: {what} must be [head_dim] of qkv's dtype and device")
+    if _custom_float(qkv):
+        _require(head_dim % 16 == 0 and head_dim <= 256,
+                 f"{name}: head_dim {head_dim} unsupported by the kernel (multiples of 16 up to 256)")
+    return (heads + kv_heads) * head_dim
+
+
+def _out_rows(name, out, like, rows, cols):
+    """``out`` checked as a row-major [rows, >= cols] matrix the kernels can write in place, or a new one."""
+    if out is None:
+        ld = (cols + 7) // 8 * 8
+        return torch.empty(rows, ld, dtype=like.dtype, device=like.device)[:, :cols]
+    ok = (out.dim() == 2 and out.shape[0] == rows and out.shape[1] >= cols and out.stride(1) == 1
+          and (rows < 2 or out.stride(0) >= cols) and out.dtype == like.dtype and out.device == like.device)
+    if _custom_float(like):
+        ok = ok and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0
+    _require(ok, f"{name}: out must be [rows, >= {cols}] row-major of the input's dtype and device, its rows on "
+                 "16-byte boundaries with a leading dimension that is a multiple of 8")
+    return out[:, :cols]
+
+
+def _gain_rows(q_gain, k_gain, heads, kv_heads, dt):
+    return torch.cat([q_gain.to(dt).expand(heads, -1), k_gain.to(dt).expand(kv_heads, -1)])
+
+
+def _rope_angles(rows, seq_len, head_dim, theta, dt, device):
+    """(cos, sin) [rows, 1, head_dim / 2]; the angles in fp64 (an fp32 angle is off by 4e-3 at position 1e5)."""
+    half = head_dim // 2
+    inv = theta ** (torch.arange(half, device=device, dtype=torch.float64) * (-2.0 / head_dim))
+    ang = (torch.arange(rows, device=device) % seq_len).double()[:, None] * inv
+    return ang.cos().to(dt)[:, None], ang.sin().to(dt)[:, None]
+
+
+def qk_norm_rope(qkv, q_gain, k_gain, seq_len: int, heads: int, kv_heads: int, head_dim: int, theta: float,
+                 eps: float = 1e-5, out: torch.Tensor | None = None) -> torch.Tensor:
+    """RMS norm of every query and key head of each row of ``qkv``, then rotate-half RoPE, in one pass.
+
+    ``qkv`` [T, >= (heads + kv_heads) * head_dim] holds the query heads, then the key heads (columns
+    behind them are not read); row t has position t % seq_len.  Each head is scaled by
+    ``(mean(x^2) + eps)^-1/2`` times ``q_gain`` / ``k_gain`` [head_dim] and rotated as ``rope_`` does.
+    Returns [T, (heads + kv_heads) * head_dim]; ``qkv`` itself is what the backward needs.
+    """
+    cols = _check_heads("qk_norm_rope", qkv, q_gain, k_gain, seq_len, heads, kv_heads, head_dim, theta, eps)
+    T = qkv.shape[0]
+    res = _out_rows("qk_norm_rope", out, qkv, T, cols)
+    if _custom_float(qkv):
+        extension().qk_norm_rope_fwd(_mat(qkv), _aligned(q_gain), _aligned(k_gain), res, seq_len, heads, kv_heads, head_dim,
+                                     theta, eps)
+        return res
+    dt, half = _acc(qkv), head_dim // 2
+    x = qkv[:, :cols].to(dt).reshape(T, -1, head_dim)
+    u = x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * _gain_rows(q_gain, k_gain, heads, kv_heads, dt)
+    cs, sn = _rope_angles(T, seq_len, head_dim, theta, dt, qkv.device)
+    a, b = u[..., :half], u[..., half:]
+    res.copy_(torch.cat([a * cs - b * sn, b * cs + a * sn], -1).reshape(T, cols))
+    return res
+
+
+def qk_norm_rope_bwd(dqk, qkv, q_gain, k_gain, seq_len: int, heads: int, kv_heads: int, head_dim: int, theta: float,
+                     dq_gain: torch.Tensor, dk_gain: torch.Tensor, eps: float = 1e-5,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of ``qk_norm_rope``: returns that of ``qkv``'s query and key columns, and adds the gains'
+    to ``dq_gain`` / ``dk_gain`` (fp32 [head_dim]).
+
+    ``dqk`` [T, >= (heads + kv_heads) * head_dim] is the gradient of the result.  ``out`` may be ``dqk``
+    itself (columns behind the heads stay as they are) or memory that does not overlap the inputs.
+    Equal inputs give equal bits.
+    """
+    cols = _check_heads("qk_norm_rope_bwd", qkv, q_gain, k_gain, seq_len, heads, kv_heads, head_dim, theta, eps)
+    T = qkv.shape[0]
+    _require(dqk.dim() == 2 and dqk.shape[0] == T and dqk.shape[1] >= cols and dqk.dtype == qkv.dtype
+             and dqk.device == qkv.device, f"qk_norm_rope_bwd: dqk must be [rows, >= {cols}] of qkv's dtype and device")
+    for g, what in ((dq_gain, "dq_gain"), (dk_gain, "dk_gain")):
+        _require(tuple(g.shape) == (head_dim,) and g.dtype == _acc(qkv) and g.device == qkv.device
+                 and g.is_contiguous(), f"qk_norm_rope_bwd: {what} must be contiguous {_acc(qkv)} [head_dim]")
+    res = _out_rows("qk_norm_rope_bwd", out, qkv, T, cols)
+    if _custom_float(qkv):
+        extension().qk_norm_rope_bwd(_mat(dqk), _mat(qkv), _aligned(q_gain), _aligned(k_gain), res, seq_len, heads, kv_heads,
+                                     head_dim, theta, eps, dq_gain, dk_gain)
+        return res
+    dt, half = _acc(qkv), head_dim // 2
+    x = qkv[:, :cols].to(dt).reshape(T, -1, head_dim)
+    dy = dqk[:, :cols].to(dt).reshape(T, -1, head_dim)
+    cs, sn = _rope_angles(T, seq_len, head_dim, theta, dt, qkv.device)
+    a, b = dy[..., :half], dy[..., half:]
+    du = torch.cat([a * cs + b * sn, b * cs - a * sn], -1)
+    r = torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps)
+    dgain = (du * x * r).sum(0)
+    dq_gain += dgain[:heads].sum(0)
+    dk_gain += dgain[heads:].sum(0)
+    w = du * _gain_rows(q_gain, k_gain, heads, kv_heads, dt)
+    dx = r * (w - x * r * (w * x * r).mean(-1, keepdim=True))
+    res.copy_(dx.reshape(T, cols))
+    return res
+
+
+# ----------------------------------------------------------------------------- dropout
+
+_U32 = 0xFFFFFFFF
+
+
+def _signed64(v: int) -> int:
+    return v - (1 << 64) if v >= 1 << 63 else v
+
+
+def _mul32(a: torch.Tensor, m: int):
+    """(high, low) 32-bit words of a * m for 32-bit values held in int64."""
+    return (a * (m >> 16) + ((a * (m & 0xFFFF)) >> 16)) >> 16, (a * m) & _U32
+
+
+def _keep_mask(shape, cut: int, seed: int, offset, device) -> torch.Tensor:
+    """The elements ``dropout`` keeps: 16 bits each of Philox4x32-10 (Salmon, Moraes, Dror, Shaw,
+    "Parallel random numbers: as easy as 1, 2, 3", 2011) at counter (element // 8, offset), key ``seed``."""
+    n = math.prod(shape)
+    g = torch.arange((n + 7) // 8, device=device)
+    off = torch.as_tensor(_signed64(offset) if isinstance(offset, int) else offset, dtype=torch.int64, device=device)
+    zero = torch.zeros_like(g)
+    c = [g & _U32, g >> 32, zero + (off & _U32), zero + ((off >> 32) & _U32)]
+    k0, k1 = seed & _U32, seed >> 32
+    for _ in range(10):
+        (h0, l0), (h1, l1) = _mul32(c[0], 0xD2511F53), _mul32(c[2], 0xCD9E8D57)
+        c = [h1 ^ c[1] ^ k0, l1, h0 ^ c[3] ^ k1, l0]
+        k0, k1 = (k0 + 0x9E3779B9) & _U32, (k1 + 0xBB67AE85) & _U32
+    words = torch.stack(c, -1)
+    bits = torch.stack([words & 0xFFFF, words >> 16], -1).reshape(-1)[:n]
+    return (bits >= cut).reshape(shape)
+
+
+def dropout(x: torch.Tensor, p: float, seed: int, offset, residual: torch.Tensor | None = None,
+            out: torch.Tensor | None = None) -> torch.Tensor:
+    """``residual + keep * x / (1 - p)``, the mask ``keep`` a function of (seed, offset, element index).
+
+    No mask is stored: the same call on the gradient of the result is the backward with respect to
+    ``x`` (the residual's gradient is the result's), and a recomputed forward repeats the mask.  ``p``
+    is taken to the nearest 1/65536, and the scale is the inverse of that exact keep probability.
+    ``seed`` and ``offset`` are 64-bit: one seed per run, another offset for every use of it.  ``offset``
+    may be a one-element int64 tensor on x's device, read when the kernel runs, so that a captured graph
+    draws another mask at each replay.  ``out`` may be ``x`` or ``residual``.  Dropped elements add
+    exactly 0, whatever ``x`` holds there.
+    """
+    _require(0.0 <= p < 1.0 and round(p * 65536) < 65536, f"dropout: p must be in [0, 1) and round below 1, got {p}")
+    cut = round(p * 65536)
+    _require(0 <= seed < 1 << 64, "dropout: seed must be a 64-bit unsigned integer")
+    on_device = isinstance(offset, torch.Tensor)
+    if on_device:
+        _require(offset.numel() == 1 and offset.dtype == torch.int64 and offset.device == x.device,
+                 "dropout: an offset tensor must be one int64 on x's device")
+        offset = offset.reshape(1)
+    else:
+        _require(0 <= offset < 1 << 64, "dropout: offset must be a 64-bit unsigned integer")
+    for t, what in ((residual, "residual"), (out, "out")):
+        _require(t is None or (t.shape == x.shape and t.dtype == x.dtype and t.device == x.device),
+                 f"dropout: {what} must have x's shape, dtype and device")
+    _require(out is None or out.is_contiguous(), "dropout: out must be contiguous")
+    if _custom_float(x):
+        _require(out is None or out.data_ptr() % 16 == 0, "dropout: out must start on a 16-byte boundary")
+        res = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+        extension().dropout(_aligned(x), None if residual is None else _aligned(residual), res, cut,
+                            _signed64(seed), 0 if on_device else _signed64(offset), offset if on_device else None)
+        return res
+    dt = _acc(x)
+    keep = _keep_mask(x.shape, cut, seed, offset, x.device)
+    y = torch.where(keep, x.to(dt) * (65536 / (65536 - cut)), 0.0)
+    if residual is not None:
+        y = residual.to(dt) + y
+    return y.to(x.dtype) if out is None else out.copy_(y)
+
+
 # ----------------------------------------------------------------------------- attention
 
 def attention(q, k, v, *, causal: bool = True, scale: float | None = None):
@@ -470,6 +682,164 @@ def cross_entropy_chunk_(logits: torch.Tensor, vocab: int, targets: torch.Tensor
     grad[torch.arange(lg.shape[0], device=lg.device), tgc] -= 1.0
     grad *= (grad_scale * valid.float())[:, None]
     logits[:, :vocab] = grad.to(logits.dtype)
+
+
+def _check_logits(name, logits, vocab, targets):
+    _require(logits.dim() == 2 and 1 <= vocab <= logits.shape[1] and logits.is_floating_point(),
+             f"{name}: logits must be [rows, >= vocab]")
+    return _vector(targets, logits.shape[0], logits, torch.int64, f"{name}: targets")
+
+
+def _rows_of(logits, vocab):
+    """The first ``vocab`` columns for the kernels; rows of narrower layouts are copied into padded ones."""
+    return _mat(logits[:, :vocab])
+
+
+def _plain_logprobs(logits, vocab, tg):
+    dt = _acc(logits)
+    lg = logits[:, :vocab].to(dt)
+    m = lg.nan_to_num(-math.inf, math.inf, -math.inf).amax(-1)
+    s = torch.exp(lg - torch.where(m == -math.inf, 0.0, m)[:, None]).sum(-1)
+    valid = (tg >= 0) & (tg < vocab)
+    lp = (lg.gather(1, tg.clamp(0, vocab - 1)[:, None])[:, 0] - m) - s.log()
+    lp = torch.where((m == -math.inf) & (s == 0), -math.inf, lp)
+    return torch.where(valid, lp, 0.0), torch.stack([m, s], -1)
+
+
+def _plain_dlogits(logits, vocab, tg, stats, dlogps, res):
+    lg = logits[:, :vocab].to(_acc(logits))
+    m, s = stats.view(-1, 2).unbind(-1)
+    at = tg.clamp(0, vocab - 1)[:, None]
+    up = torch.where((tg == at[:, 0]) & ~((m == -math.inf) & (s == 0)), dlogps, 0.0)
+    d = -torch.exp(lg - torch.where(m == -math.inf, 0.0, m)[:, None]) / s[:, None]
+    d.scatter_add_(1, at, torch.ones_like(up)[:, None])
+    res.copy_(torch.where((up == 0)[:, None], 0.0, d * up[:, None]))
+    return res
+
+
+def token_logprobs(logits: torch.Tensor, vocab: int, targets: torch.Tensor):
+    """(logps [T], stats [T, 2]), fp32: the log probability of each row's target, and the row's maximum m
+    and sum of exp(x - m), which the backward takes (log-sum-exp = m + log of the sum).
+
+    ``logits`` [T, >= vocab] as the LM head's GEMM leaves them.  A target outside [0, vocab) marks a row
+    without a token: logp 0.  A row whose logits are all -inf has m = logp = -inf and the sum 0.
+    """
+    tg = _check_logits("token_logprobs", logits, vocab, targets)
+    if _custom_float(logits):
+        return tuple(extension().token_logprobs(_rows_of(logits, vocab), vocab, tg))
+    return _plain_logprobs(logits, vocab, tg)
+
+
+def token_logprobs_bwd(logits: torch.Tensor, vocab: int, targets: torch.Tensor, stats: torch.Tensor,
+                       dlogps: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of the logits from that of ``token_logprobs``'s logps: (onehot - softmax) * dlogps.
+    ``stats`` is what ``token_logprobs`` returned for these logits.
+
+    Rows without a token, rows whose ``dlogps`` is 0 and rows of nothing but -inf get zeros whatever they
+    hold.  ``out`` may be ``logits`` (overwritten); otherwise a new matrix, whose rows are padded
+    to a multiple of 8 columns as the LM head's GEMMs take them.  Returns its first ``vocab`` columns.
+    """
+    tg = _check_logits("token_logprobs_bwd", logits, vocab, targets)
+    T, dt = logits.shape[0], _acc(logits)
+    stats = _vector(stats, 2 * T, logits, dt, "token_logprobs_bwd: stats")
+    dlogps = _vector(dlogps, T, logits, dt, "token_logprobs_bwd: dlogps")
+    res = _out_rows("token_logprobs_bwd", out, logits, T, vocab)
+    if _custom_float(logits):
+        extension().token_logprobs_bwd(_rows_of(logits, vocab), vocab, tg, _aligned(stats), dlogps, res)
+        return res
+    return _plain_dlogits(logits, vocab, tg, stats, dlogps, res)
+
+
+def policy_loss_chunk(logits: torch.Tensor, vocab: int, targets: torch.Tensor, old_logps: torch.Tensor,
+                      advantages: torch.Tensor, weights: torch.Tensor | None = None, *,
+                      ref_logps: torch.Tensor | None = None, clip_low: float = 0.2, clip_high: float = 0.2,
+                      kl_coef: float = 0.0, grad_scale: float = 1.0, out: torch.Tensor | None = None):
+    """Clipped policy loss of sampled tokens with a KL term, forward and backward in one pass over the logits.
+
+    Per row, with logp the log probability of its target and rho = exp(logp - old_logps):
+
+        loss = weights * (max(-A rho, -A clip(rho, 1 - clip_low, 1 + clip_high))
+                          + kl_coef * (exp(d) - d - 1)),    A = advantages, d = ref_logps - logp
+
+    ``weights`` carry the mask and the normalisation (mask / tokens for a mean over tokens; None: 1).
+    A row of weight 0 or whose target is outside [0, vocab) has loss 0 and gradient 0 whatever it holds.
+    Where both sides of the max are equal the gradient is the unclipped side's.  Returns (losses [T],
+    logps [T], dlogits), the last the gradient of ``grad_scale * sum(losses)``; ``out`` as in
+    ``token_logprobs_bwd``.  All per-row tensors are fp32 [T].
+    """
+    name = "policy_loss_chunk"
+    tg = _check_logits(name, logits, vocab, targets)
+    T, dt = logits.shape[0], _acc(logits)
+    old, adv, w, ref = (None if t is None else _vector(t, T, logits, dt, f"{name}: {n}") for t, n in (
+        (old_logps, "old_logps"), (advantages, "advantages"), (weights, "weights"), (ref_logps, "ref_logps")))
+    _require(0.0 <= clip_low <= 1.0 and clip_high >= 0.0, f"{name}: needs 0 <= clip_low <= 1 and clip_high >= 0")
+    _require(kl_coef == 0.0 or ref is not None, f"{name}: a KL term needs ref_logps")
+    if kl_coef == 0.0:
+        ref = None
+    res = _out_rows(name, out, logits, T, vocab)
+    if _custom_float(logits):
+        losses, logps = extension().policy_loss(_rows_of(logits, vocab), vocab, tg, old, ref, adv, w, clip_low,
+                                                clip_high, kl_coef, grad_scale, res)
+        return losses, logps, res
+    lp, stats = _plain_logprobs(logits, vocab, tg)
+    valid = (tg >= 0) & (tg < vocab)
+    lpd = lp.double()
+    ratio = torch.exp(lpd - old)
+    free, bound = -adv * ratio, -adv * ratio.clamp(1.0 - clip_low, 1.0 + clip_high)
+    loss = torch.maximum(free, bound)
+    d = torch.where((free >= bound) | free.isnan(), free, 0.0)
+    if ref is not None:
+        back = ref - lpd
+        loss = loss + kl_coef * (torch.expm1(back) - back)
+        d = d - kl_coef * torch.expm1(back)
+    if w is not None:
+        valid = valid & (w != 0)
+        loss, d = loss * w, d * w
+    loss = torch.where(valid, loss, 0.0).to(dt)
+    dlogps = torch.where(valid, d * grad_scale, 0.0).to(dt)
+    return loss, lp, _plain_dlogits(logits, vocab, tg, stats, dlogps, res)
+
+
+def preference_loss(logps: torch.Tensor, ref_logps: torch.Tensor, mask: torch.Tensor, beta: float = 0.1, *,
+                    form: str = "sigmoid", label_smoothing: float = 0.0, grad_scale: float = 1.0):
+    """Preference loss of pairs of answers from the log ratios of their tokens, and its gradient.
+
+    ``logps`` and ``ref_logps`` [2 P, S] fp32 are the tokens' log probabilities under the trained and the
+    reference model; rows 2i and 2i + 1 are pair i's preferred and rejected answer; ``mask`` [2 P, S]
+    bool marks the tokens that count.  With r the masked sum of logps - ref_logps of a row and n its count:
+
+        sigmoid:  h = beta (r_0 - r_1),  loss = -(1 - s) log sigma(h) - s log sigma(-h),  s = label_smoothing
+        squared:  loss = (r_0 / n_0 - r_1 / n_1 - 1 / (2 beta))^2
+
+    An empty row has r = 0 and no gradient.  Returns (losses [P], rewards [2 P] = beta r, dlogps [2 P, S],
+    the gradient of ``grad_scale * sum(losses)``).  Masked tokens are not looked at.
+    """
+    dt = _acc(logps)
+    _require(logps.dim() == 2 and logps.shape[0] % 2 == 0 and logps.dtype == dt,
+             "preference_loss: logps must be fp32 [2 pairs, S]")
+    _require(form in ("sigmoid", "squared"), f"preference_loss: unknown form {form!r} (sigmoid, squared)")
+    _require(beta > 0 and 0.0 <= label_smoothing <= 1.0, "preference_loss: needs beta > 0 and 0 <= label_smoothing <= 1")
+    _require(form == "sigmoid" or label_smoothing == 0.0, "preference_loss: label_smoothing is the sigmoid form's")
+    for t, n, want in ((ref_logps, "ref_logps", dt), (mask, "mask", torch.bool)):
+        _require(t.shape == logps.shape and t.dtype == want and t.device == logps.device,
+                 f"preference_loss: {n} must be {want} with logps's shape and device")
+    if _custom_float(logps):
+        return tuple(extension().preference_loss(logps.contiguous(), ref_logps.contiguous(), mask.contiguous(), beta,
+                                                 label_smoothing, form == "squared", grad_scale))
+    r = torch.where(mask, logps.double() - ref_logps, 0.0).sum(-1)
+    r0, r1 = r[0::2], r[1::2]
+    if form == "sigmoid":
+        h = beta * (r0 - r1)
+        losses = -(1 - label_smoothing) * F.logsigmoid(h) - label_smoothing * F.logsigmoid(-h)
+        up = beta * (label_smoothing - torch.sigmoid(-h))
+        up = torch.stack([up, -up], -1).reshape(-1)
+    else:
+        n = mask.sum(-1).clamp(min=1)
+        gap = r0 / n[0::2] - r1 / n[1::2] - 0.5 / beta
+        losses = gap.square()
+        up = torch.stack([2 * gap, -2 * gap], -1).reshape(-1) / n
+    dlogps = torch.where(mask, (up * grad_scale)[:, None], 0.0).to(dt)
+    return losses.to(dt), (beta * r).to(dt), dlogps
 
 
 # ----------------------------------------------------------------------------- optimizer

@@ -247,6 +247,219 @@ void cross_entropy_(Tensor logits, int64_t V, Tensor targets, Tensor loss_sum, d
                   "cross_entropy");
 }
 
+// Element type code of mt_api.h.
+int dtype_code(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return 0;
+    case at::kHalf: return 1;
+    case at::kFloat: return 2;
+    default: TORCH_CHECK(false, name, " has dtype ", t.scalar_type(), ", expected bfloat16, float16 or float32");
+  }
+  return -1;
+}
+// A row-major matrix whose rows start on 16-byte boundaries, on `like`'s device and of its type.
+void check_rows_like(const Tensor& t, const char* name, const Tensor& like, int64_t rows, int64_t cols) {
+  TORCH_CHECK(t.is_cuda() && t.get_device() == like.get_device(), name, " must be on ", like.device());
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " has dtype ", t.scalar_type(), ", expected ",
+              like.scalar_type());
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) >= cols && t.stride(1) == 1, name, " must be [", rows,
+              ", >= ", cols, "] row-major");
+  TORCH_CHECK(rows < 2 || t.stride(0) >= cols, name, " rows overlap");
+  TORCH_CHECK(rows < INT32_MAX && cols < INT32_MAX, name, " is too large");
+  TORCH_CHECK(t.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0, name,
+              " rows must be 16-byte aligned with a leading dimension that is a multiple of 8");
+}
+// A contiguous vector of n values on `like`'s device.
+void check_vector(const Tensor& t, const char* name, at::ScalarType dt, const Tensor& like, int64_t n) {
+  check_cuda(t, name, dt);
+  TORCH_CHECK(t.get_device() == like.get_device(), name, " must be on ", like.device());
+  TORCH_CHECK(t.is_contiguous() && t.numel() == n, name, " must be contiguous with ", n, " values");
+}
+
+mt::QkNormRopeArgs qk_args(const Tensor& x, const Tensor& gq, const Tensor& gk, const Tensor& out, int64_t S, int64_t H,
+                           int64_t HK, int64_t hd, double theta, double eps) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, "qk_norm_rope: qkv must be a CUDA matrix");
+  const int code = dtype_code(x, "qkv");
+  TORCH_CHECK(hd % 16 == 0 && hd >= 16 && hd <= 256, "qk_norm_rope: head_dim ", hd,
+              " unsupported (multiples of 16 up to 256)");
+  TORCH_CHECK(H >= 0 && HK >= 0 && H + HK >= 1 && H + HK <= 65536 && S >= 1 && S < INT32_MAX,
+              "qk_norm_rope: bad heads or seq_len");
+  TORCH_CHECK(theta > 0 && eps >= 0, "qk_norm_rope: theta must be positive and eps not negative");
+  const int64_t rows = x.size(0), cols = (H + HK) * hd;
+  check_rows_like(x, "qkv", x, rows, cols);
+  check_rows_like(out, "out", x, rows, cols);
+  check_vector(gq, "q_gain", x.scalar_type(), x, hd);
+  check_vector(gk, "k_gain", x.scalar_type(), x, hd);
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(gq.data_ptr()) & 15) == 0 &&
+                  (reinterpret_cast<uintptr_t>(gk.data_ptr()) & 15) == 0,
+              "qk_norm_rope: gains must be 16-byte aligned");
+  mt::QkNormRopeArgs a{};
+  a.x = x.data_ptr();
+  a.ldx = x.stride(0);
+  a.gq = gq.data_ptr();
+  a.gk = gk.data_ptr();
+  a.out = out.data_ptr();
+  a.ldo = out.stride(0);
+  a.dtype = code;
+  a.rows = (int)rows;
+  a.S = (int)S;
+  a.H = (int)H;
+  a.HK = (int)HK;
+  a.hd = (int)hd;
+  a.eps = (float)eps;
+  a.theta = theta;
+  return a;
+}
+
+void qk_norm_rope_fwd(Tensor x, Tensor gq, Tensor gk, Tensor out, int64_t S, int64_t H, int64_t HK, int64_t hd,
+                      double theta, double eps) {
+  const mt::QkNormRopeArgs a = qk_args(x, gq, gk, out, S, H, HK, hd, theta, eps);
+  c10::cuda::CUDAGuard guard(x.get_device());
+  MT_CHECK_LAUNCH(mt::qk_norm_rope_fwd(a, stream_of(x)), "qk_norm_rope");
+}
+
+void qk_norm_rope_bwd(Tensor dy, Tensor x, Tensor gq, Tensor gk, Tensor out, int64_t S, int64_t H, int64_t HK,
+                      int64_t hd, double theta, double eps, Tensor dgq, Tensor dgk) {
+  const mt::QkNormRopeArgs a = qk_args(x, gq, gk, out, S, H, HK, hd, theta, eps);
+  check_rows_like(dy, "dqk", x, x.size(0), (H + HK) * hd);
+  check_vector(dgq, "dq_gain", at::kFloat, x, hd);
+  check_vector(dgk, "dk_gain", at::kFloat, x, hd);
+  if (a.rows == 0) return;
+  c10::cuda::CUDAGuard guard(x.get_device());
+  auto partial = torch::empty({mt::qk_norm_rope_blocks(a.rows, a.H + a.HK, a.hd), 2 * hd},
+                              x.options().dtype(at::kFloat));
+  MT_CHECK_LAUNCH(mt::qk_norm_rope_bwd(a, dy.data_ptr(), dy.stride(0), partial.data_ptr<float>(),
+                                       dgq.data_ptr<float>(), dgk.data_ptr<float>(), stream_of(x)),
+                  "qk_norm_rope_bwd");
+}
+
+// seed and offset carry 64 unsigned bits in int64.
+void dropout(Tensor x, c10::optional<Tensor> residual, Tensor out, int64_t cut, int64_t seed, int64_t offset,
+             c10::optional<Tensor> offset_tensor) {
+  TORCH_CHECK(x.is_cuda(), "dropout: x must be a CUDA tensor");
+  mt::DropoutArgs a{};
+  a.dtype = dtype_code(x, "x");
+  check_rows(x, "x");
+  a.x = x.data_ptr();
+  a.n = x.numel();
+  for (auto* t : {residual ? &*residual : &x, &out}) {
+    TORCH_CHECK(t->is_cuda() && t->get_device() == x.get_device() && t->scalar_type() == x.scalar_type() &&
+                    t->numel() == x.numel(),
+                "dropout: residual and out must have x's device, dtype and size");
+    check_rows(*t, "dropout: residual and out");
+  }
+  if (residual) a.residual = residual->data_ptr();
+  a.out = out.data_ptr();
+  TORCH_CHECK(cut >= 0 && cut < 65536, "dropout: p must round to less than 1");
+  a.cut = (uint32_t)cut;
+  a.seed = (uint64_t)seed;
+  a.offset = (uint64_t)offset;
+  if (offset_tensor) {
+    check_vector(*offset_tensor, "offset", at::kLong, x, 1);
+    a.offset_ptr = offset_tensor->data_ptr<int64_t>();
+  }
+  c10::cuda::CUDAGuard guard(x.get_device());
+  MT_CHECK_LAUNCH(mt::dropout_apply(a, stream_of(x)), "dropout");
+}
+
+void check_logits(const Tensor& logits, int64_t V, const Tensor& targets) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && V >= 1, "logits must be a CUDA matrix [rows, >= vocab]");
+  check_rows_like(logits, "logits", logits, logits.size(0), V);
+  check_vector(targets, "targets", at::kLong, logits, logits.size(0));
+}
+
+std::vector<Tensor> token_logprobs(Tensor logits, int64_t V, Tensor targets) {
+  check_logits(logits, V, targets);
+  const int64_t rows = logits.size(0);
+  c10::cuda::CUDAGuard guard(logits.get_device());
+  auto fopts = logits.options().dtype(at::kFloat);
+  auto logps = torch::empty({rows}, fopts), stats = torch::empty({rows, 2}, fopts);
+  MT_CHECK_LAUNCH(mt::token_logprobs(logits.data_ptr(), logits.stride(0), dtype_code(logits, "logits"),
+                                     targets.data_ptr<int64_t>(), logps.data_ptr<float>(), stats.data_ptr<float>(),
+                                     (int)rows, (int)V, stream_of(logits)),
+                  "token_logprobs");
+  return {logps, stats};
+}
+
+void token_logprobs_bwd(Tensor logits, int64_t V, Tensor targets, Tensor stats, Tensor dlogps, Tensor out) {
+  check_logits(logits, V, targets);
+  const int64_t rows = logits.size(0);
+  check_vector(stats, "stats", at::kFloat, logits, 2 * rows);
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(stats.data_ptr()) & 7) == 0, "stats must be 8-byte aligned");
+  check_vector(dlogps, "dlogps", at::kFloat, logits, rows);
+  check_rows_like(out, "out", logits, rows, V);
+  c10::cuda::CUDAGuard guard(logits.get_device());
+  MT_CHECK_LAUNCH(mt::token_logprobs_bwd(logits.data_ptr(), logits.stride(0), dtype_code(logits, "logits"),
+                                         targets.data_ptr<int64_t>(), stats.data_ptr<float>(),
+                                         dlogps.data_ptr<float>(), out.data_ptr(), out.stride(0), (int)rows, (int)V,
+                                         stream_of(logits)),
+                  "token_logprobs_bwd");
+}
+
+std::vector<Tensor> policy_loss(Tensor logits, int64_t V, Tensor targets, Tensor old_logps,
+                                c10::optional<Tensor> ref_logps, Tensor advantages, c10::optional<Tensor> weights,
+                                double clip_low, double clip_high, double kl_coef, double grad_scale, Tensor out) {
+  check_logits(logits, V, targets);
+  const int64_t rows = logits.size(0);
+  check_vector(old_logps, "old_logps", at::kFloat, logits, rows);
+  check_vector(advantages, "advantages", at::kFloat, logits, rows);
+  if (ref_logps) check_vector(*ref_logps, "ref_logps", at::kFloat, logits, rows);
+  if (weights) check_vector(*weights, "weights", at::kFloat, logits, rows);
+  check_rows_like(out, "out", logits, rows, V);
+  c10::cuda::CUDAGuard guard(logits.get_device());
+  auto losses = torch::empty({rows}, logits.options().dtype(at::kFloat)), logps = torch::empty_like(losses);
+  mt::PolicyArgs a{};
+  a.logits = logits.data_ptr();
+  a.ld = logits.stride(0);
+  a.out = out.data_ptr();
+  a.ldo = out.stride(0);
+  a.dtype = dtype_code(logits, "logits");
+  a.targets = targets.data_ptr<int64_t>();
+  a.old_logps = old_logps.data_ptr<float>();
+  a.ref_logps = ref_logps ? ref_logps->data_ptr<float>() : nullptr;
+  a.advantages = advantages.data_ptr<float>();
+  a.weights = weights ? weights->data_ptr<float>() : nullptr;
+  a.losses = losses.data_ptr<float>();
+  a.logps = logps.data_ptr<float>();
+  a.rows = (int)rows;
+  a.V = (int)V;
+  a.clip_low = clip_low;
+  a.clip_high = clip_high;
+  a.kl_coef = kl_coef;
+  a.grad_scale = grad_scale;
+  MT_CHECK_LAUNCH(mt::policy_loss(a, stream_of(logits)), "policy_loss");
+  return {losses, logps};
+}
+
+std::vector<Tensor> preference_loss(Tensor logps, Tensor ref_logps, Tensor mask, double beta, double label_smoothing,
+                                    bool squared, double grad_scale) {
+  check_cuda(logps, "logps", at::kFloat);
+  TORCH_CHECK(logps.dim() == 2 && logps.size(0) % 2 == 0 && logps.size(1) < INT32_MAX && logps.is_contiguous(),
+              "preference_loss: logps must be contiguous [2 pairs, S]");
+  check_vector(ref_logps, "ref_logps", at::kFloat, logps, logps.numel());
+  check_vector(mask, "mask", at::kBool, logps, logps.numel());
+  const int64_t pairs = logps.size(0) / 2;
+  TORCH_CHECK(pairs < INT32_MAX, "preference_loss: too many pairs");
+  c10::cuda::CUDAGuard guard(logps.get_device());
+  auto losses = torch::empty({pairs}, logps.options()), rewards = torch::empty({2 * pairs}, logps.options());
+  auto dlogps = torch::empty_like(logps);
+  mt::PreferenceArgs a{};
+  a.logps = logps.data_ptr<float>();
+  a.ref_logps = ref_logps.data_ptr<float>();
+  a.mask = reinterpret_cast<const uint8_t*>(mask.data_ptr<bool>());
+  a.losses = losses.data_ptr<float>();
+  a.rewards = rewards.data_ptr<float>();
+  a.dlogps = dlogps.data_ptr<float>();
+  a.pairs = (int)pairs;
+  a.S = (int)logps.size(1);
+  a.beta = beta;
+  a.label_smoothing = label_smoothing;
+  a.grad_scale = grad_scale;
+  a.squared = squared;
+  MT_CHECK_LAUNCH(mt::preference_loss(a, stream_of(logps)), "preference_loss");
+  return {losses, rewards, dlogps};
+}
+
 void adam_(Tensor p, Tensor g, Tensor m, Tensor v, c10::optional<Tensor> pb, double lr, double beta1, double beta2,
            double eps, double wd, bool decoupled, double bc1, double bc2, double grad_scale) {
   for (auto* t : {&p, &g, &m, &v}) {
@@ -390,6 +603,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("swiglu_bwd", &swiglu_bwd);
   m.def("rope_", &rope_);
   m.def("cross_entropy_", &cross_entropy_);
+  m.def("qk_norm_rope_fwd", &qk_norm_rope_fwd);
+  m.def("qk_norm_rope_bwd", &qk_norm_rope_bwd);
+  m.def("dropout", &dropout);
+  m.def("token_logprobs", &token_logprobs);
+  m.def("token_logprobs_bwd", &token_logprobs_bwd);
+  m.def("policy_loss", &policy_loss);
+  m.def("preference_loss", &preference_loss);
   m.def("adam_", &adam_);
   m.def("cast_bf16_", &cast_bf16_);
   m.def("attention_fwd", &attention_fwd);

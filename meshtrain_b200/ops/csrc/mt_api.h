@@ -78,6 +78,82 @@ int rope_apply(void* qk, long ld, int T, int S, int H, int hd, float theta, bool
 int cross_entropy_fwd_bwd(void* logits, long ld, const int64_t* targets, float* loss_sum, int T, int V,
                           float loss_scale, float grad_scale, cudaStream_t s);
 
+// Element types of the kernels below: 0 bf16, 1 fp16, 2 fp32.
+
+// logps[r] = log softmax of logits[r, targets[r]]; stats[2 r], stats[2 r + 1] = the row's maximum m and
+// sum of exp(x - m).  Rows of width V, leading dimension ld (a multiple of 8).
+int token_logprobs(const void* logits, long ld, int dtype, const int64_t* targets, float* logps, float* stats, int rows,
+                   int V, cudaStream_t s);
+// out[r, c] = dlogps[r] * ([c == targets[r]] - softmax(logits[r])[c]); out may be logits.
+int token_logprobs_bwd(const void* logits, long ld, int dtype, const int64_t* targets, const float* stats,
+                       const float* dlogps, void* out, long ldo, int rows, int V, cudaStream_t s);
+// Clipped policy loss with a KL term, logits to loss, log probability and gradient in one pass; out may be logits.
+struct PolicyArgs {
+  const void* logits;
+  long ld;
+  void* out;
+  long ldo;
+  int dtype;
+  const int64_t* targets;
+  const float* old_logps;
+  const float* ref_logps;  // or null: no KL term
+  const float* advantages;
+  const float* weights;    // or null: 1 for every row
+  float* losses;
+  float* logps;
+  int rows, V;
+  double clip_low, clip_high, kl_coef, grad_scale;
+};
+int policy_loss(const PolicyArgs& args, cudaStream_t s);
+// Loss of pairs of answers (rows 2i preferred, 2i + 1 rejected) of S tokens and its gradient.
+struct PreferenceArgs {
+  const float* logps;      // [2 pairs, S]
+  const float* ref_logps;  // [2 pairs, S]
+  const uint8_t* mask;     // [2 pairs, S]: nonzero where a token counts
+  float* losses;           // [pairs]
+  float* rewards;          // [2 pairs]
+  float* dlogps;           // [2 pairs, S]
+  int pairs, S;
+  double beta, label_smoothing, grad_scale;
+  bool squared;
+};
+int preference_loss(const PreferenceArgs& args, cudaStream_t s);
+
+// ------------------------------------------------------------------ head norms and rotation
+// RMS norm of the H query and HK key heads (hd values, a multiple of 16 up to 256) of each row of x
+// and their rotary embedding at position row % S, into rows of `out`.
+struct QkNormRopeArgs {
+  const void* x;  // [rows, >= (H + HK) hd], row stride ldx (elements)
+  long ldx;
+  const void* gq;  // [hd]
+  const void* gk;
+  void* out;  // [rows, >= (H + HK) hd], row stride ldo: the result, or in the backward dx
+  long ldo;
+  int dtype;
+  int rows, S, H, HK, hd;
+  float eps;
+  double theta;
+};
+int qk_norm_rope_fwd(const QkNormRopeArgs& args, cudaStream_t s);
+// Blocks of the backward, each of which writes 2 hd floats of `partial`.
+int qk_norm_rope_blocks(int rows, int heads, int hd);
+// args.out = gradient of x (may be dy); dgq / dgk += gradients of the gains.
+int qk_norm_rope_bwd(const QkNormRopeArgs& args, const void* dy, long lddy, float* partial, float* dgq, float* dgk,
+                     cudaStream_t s);
+
+// ------------------------------------------------------------------ dropout
+struct DropoutArgs {
+  const void* x;
+  const void* residual;  // or null
+  void* out;             // may be x or residual
+  long n;
+  int dtype;
+  uint32_t cut;  // an element is kept if its 16 random bits are >= cut; cut < 65536
+  uint64_t seed, offset;
+  const int64_t* offset_ptr;  // or null: a device scalar added to offset
+};
+int dropout_apply(const DropoutArgs& args, cudaStream_t s);
+
 // ------------------------------------------------------------------ optimizer
 // Fused Adam/AdamW over flat fp32 arrays; optional bf16 copy-out of the params.
 int adam_step(float* param, const float* grad, float* exp_avg, float* exp_avg_sq, void* param_bf16, long n, float lr,

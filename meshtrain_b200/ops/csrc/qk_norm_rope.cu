@@ -1,0 +1,370 @@
+// qk_norm_rope.cu -- RMS norm of every query and key head and its rotation, in one pass, and its backward.
+//
+// Head x (n values) of a row at position p = row mod S, gain g, half = n/2:
+//   r = (mean(x^2) + eps)^(-1/2)      u = x r g      angle_i = p theta^(-2i/n)
+//   y_i = u_i cos_i - u_{i+half} sin_i               y_{i+half} = u_{i+half} cos_i + u_i sin_i
+// and backward from dy (r is formed again from x, which has to be read anyway):
+//   du = the inverse rotation of dy   dg += sum over rows and heads of du x r
+//   w = du g                          dx = r (w - x r mean(w x r))
+// Sums, r and the rotation are fp32, each output is rounded once.  Angles are formed in fp64 and
+// reduced to a fraction of a turn before the fp32 sine: at position 10^5 an fp32 angle is off by up
+// to 4e-3 rad, more than a bf16 rounding.
+//
+// Bound: DRAM (forward reads and writes each head once, backward reads two and writes one).  A head
+// is spread over G lanes, each holding 8 adjacent values of either half, so that the rotation's pairs
+// meet in one thread, every access is a 16-byte vector and a norm is log2(G) shuffles.  A warp takes
+// one row (or a share of its heads when there are few rows) and computes the row's sines once for
+// all heads.
+#include <cuda_runtime.h>
+#include <math.h>
+
+#include <algorithm>
+
+#include "mt_api.h"
+#include "vec_io.cuh"
+
+namespace mt {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kMaxHalf = 128;
+
+// theta^(-2i/n) / (2 pi) as a product of the powers 2^k of the ratio theta^(-2/n): the host forms
+// eight powers in fp64, a thread multiplies those of i's bits.
+struct Turns {
+  double unit;      // 1 / (2 pi)
+  double ratio[7];  // theta^(-2/n * 2^k)
+};
+
+__device__ __forceinline__ double turns_per_position(const Turns& t, int i) {
+  double f = t.unit;
+#pragma unroll
+  for (int k = 0; k < 7; ++k)
+    if (i >> k & 1) f *= t.ratio[k];
+  return f;
+}
+
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The (cos, sin) of a row's position for all pairs, into this warp's shared rows.
+__device__ __forceinline__ void row_turns(const double* freq, float* cs, float* sn, int half, int pos, int lane) {
+  __syncwarp();
+  for (int i = lane; i < half; i += 32) {
+    double t = (double)pos * freq[i];
+    t -= rint(t);
+    sincospif(2.0f * (float)t, &sn[i], &cs[i]);
+  }
+  __syncwarp();
+}
+
+template <class T, int G, int U>
+__global__ void __launch_bounds__(kWarps * 32)
+    qk_norm_rope_fwd_kernel(const T* __restrict__ x, long ldx, const T* __restrict__ gq, const T* __restrict__ gk,
+                            T* __restrict__ y, long ldy, int rows, int S, int H, int HK, int hd, float eps,
+                            int warps_per_row, Turns turns) {
+  __shared__ double freq[kMaxHalf];
+  __shared__ float cs_all[kWarps][kMaxHalf], sn_all[kWarps][kMaxHalf];
+  const int half = hd >> 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < half; i += blockDim.x) freq[i] = turns_per_position(turns, i);
+  __syncthreads();
+  const int d = (lane % G) * 8;  // this lane's values: d .. d+7 and half+d .. half+d+7
+  const bool on = d < half;
+  const int slots = (32 / G) * warps_per_row;
+  const int slot = (warp % warps_per_row) * (32 / G) + lane / G;
+  const int rows_per_block = kWarps / warps_per_row;
+  const float inv_n = 1.0f / (float)hd;
+  for (long row = (long)blockIdx.x * rows_per_block + warp / warps_per_row; row < rows;
+       row += (long)gridDim.x * rows_per_block) {
+    row_turns(freq, cs_all[warp], sn_all[warp], half, (int)(row % S), lane);
+    float cs[8], sn[8];
+    if (on) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        cs[j] = cs_all[warp][d + j];
+        sn[j] = sn_all[warp][d + j];
+      }
+    }
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {
+      const int n = part ? HK : H;
+      const T* gain = part ? gk : gq;
+      const T* xr = x + row * ldx + (part ? (long)H * hd : 0) + d;
+      T* yr = y + row * ldy + (part ? (long)H * hd : 0) + d;
+      float ga[8], gb[8];
+      if (on) {
+        load8(gain + d, ga);
+        load8(gain + half + d, gb);
+      }
+      // every lane runs the same number of turns: the shuffles need the whole warp
+      for (int h0 = 0; h0 < n; h0 += slots * U) {
+        Raw8<T> ra[U], rb[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * slots + slot;
+          if (on && h < n) {
+            ra[u] = ldraw8(xr + (long)h * hd);
+            rb[u] = ldraw8(xr + (long)h * hd + half);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * slots + slot;
+          const bool mine = on && h < n;
+          float a[8], b[8], ss = 0.f;
+          if (mine) {
+            unpack8(ra[u], a);
+            unpack8(rb[u], b);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ss += a[j] * a[j] + b[j] * b[j];
+          }
+          const float r = rsqrtf(group_sum<G>(ss) * inv_n + eps);
+          if (mine) {
+            float o1[8], o2[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float ua = a[j] * r * ga[j], ub = b[j] * r * gb[j];
+              o1[j] = ua * cs[j] - ub * sn[j];
+              o2[j] = ub * cs[j] + ua * sn[j];
+            }
+            store8(yr + (long)h * hd, o1);
+            store8(yr + (long)h * hd + half, o2);
+          }
+        }
+      }
+    }
+  }
+}
+
+// The gain gradients of a block go to its row of `partial` [blocks][2][hd]; gain_sum_kernel adds the
+// rows in a fixed order, so that equal inputs give equal bits.
+template <class T, int G, int U>
+__global__ void __launch_bounds__(kWarps * 32)
+    qk_norm_rope_bwd_kernel(const T* dy, long lddy, const T* __restrict__ x, long ldx, const T* __restrict__ gq,
+                            const T* __restrict__ gk, T* dx, long lddx, float* __restrict__ partial, int rows, int S,
+                            int H, int HK, int hd, float eps, int warps_per_row, Turns turns) {
+  __shared__ double freq[kMaxHalf];
+  __shared__ float cs_all[kWarps][kMaxHalf], sn_all[kWarps][kMaxHalf];
+  __shared__ float red[kWarps][2 * kMaxHalf];
+  const int half = hd >> 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < half; i += blockDim.x) freq[i] = turns_per_position(turns, i);
+  __syncthreads();
+  const int d = (lane % G) * 8;
+  const bool on = d < half;
+  const int slots = (32 / G) * warps_per_row;
+  const int slot = (warp % warps_per_row) * (32 / G) + lane / G;
+  const int rows_per_block = kWarps / warps_per_row;
+  const float inv_n = 1.0f / (float)hd;
+  float acc[2][16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) acc[0][j] = acc[1][j] = 0.f;
+  for (long row = (long)blockIdx.x * rows_per_block + warp / warps_per_row; row < rows;
+       row += (long)gridDim.x * rows_per_block) {
+    row_turns(freq, cs_all[warp], sn_all[warp], half, (int)(row % S), lane);
+    float cs[8], sn[8];
+    if (on) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        cs[j] = cs_all[warp][d + j];
+        sn[j] = sn_all[warp][d + j];
+      }
+    }
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const int n = part ? HK : H;
+      const T* gain = part ? gk : gq;
+      const long head0 = part ? (long)H * hd : 0;
+      const T* xr = x + row * ldx + head0 + d;
+      const T* gr = dy + row * lddy + head0 + d;
+      T* dxr = dx + row * lddx + head0 + d;
+      float ga[8], gb[8];
+      if (on) {
+        load8(gain + d, ga);
+        load8(gain + half + d, gb);
+      }
+      for (int h0 = 0; h0 < n; h0 += slots * U) {
+        Raw8<T> xa[U], xb[U], ya[U], yb[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * slots + slot;
+          if (on && h < n) {
+            xa[u] = ldraw8(xr + (long)h * hd);
+            xb[u] = ldraw8(xr + (long)h * hd + half);
+            ya[u] = ldraw8(gr + (long)h * hd);
+            yb[u] = ldraw8(gr + (long)h * hd + half);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int h = h0 + u * slots + slot;
+          const bool mine = on && h < n;
+          float a[8], b[8], va[8], vb[8], ss = 0.f, dot = 0.f;
+          if (mine) {
+            float ea[8], eb[8];
+            unpack8(xa[u], a);
+            unpack8(xb[u], b);
+            unpack8(ya[u], ea);
+            unpack8(yb[u], eb);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              va[j] = ea[j] * cs[j] + eb[j] * sn[j];
+              vb[j] = eb[j] * cs[j] - ea[j] * sn[j];
+              ss += a[j] * a[j] + b[j] * b[j];
+              dot += va[j] * ga[j] * a[j] + vb[j] * gb[j] * b[j];
+            }
+          }
+          const float r = rsqrtf(group_sum<G>(ss) * inv_n + eps);
+          const float m = group_sum<G>(dot) * inv_n * r * r;  // mean(w x r) r
+          if (mine) {
+            float o1[8], o2[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              acc[part][j] += va[j] * a[j] * r;
+              acc[part][8 + j] += vb[j] * b[j] * r;
+              o1[j] = r * (va[j] * ga[j] - a[j] * m);
+              o2[j] = r * (vb[j] * gb[j] - b[j] * m);
+            }
+            store8(dxr + (long)h * hd, o1);
+            store8(dxr + (long)h * hd + half, o2);
+          }
+        }
+      }
+    }
+  }
+  // lanes that hold the same columns, then the block's warps, in a fixed order
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      float v = acc[part][j];
+#pragma unroll
+      for (int o = 16; o >= G; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane < G && on) red[warp][(j < 8 ? 0 : half) + d + (j & 7)] = v;
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < hd; c += blockDim.x) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) s += red[w][c];
+      partial[((long)blockIdx.x * 2 + part) * hd + c] = s;
+    }
+    __syncthreads();
+  }
+}
+
+constexpr int kSumCols = 32, kSumGroups = 32;
+
+__global__ void __launch_bounds__(kSumCols * kSumGroups)
+    gain_sum_kernel(const float* __restrict__ partial, int blocks, int hd, float* __restrict__ dgq,
+                    float* __restrict__ dgk) {
+  __shared__ float part[kSumGroups][kSumCols + 1];
+  const int c = threadIdx.x % kSumCols, g = threadIdx.x / kSumCols;
+  const int col = blockIdx.x * kSumCols + c;  // of 2 hd; hd is a multiple of 16
+  float s = 0.f;
+  if (col < 2 * hd)
+    for (int b = g; b < blocks; b += kSumGroups) s += partial[(long)b * 2 * hd + col];
+  part[g][c] = s;
+  __syncthreads();
+  if (g == 0 && col < 2 * hd) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < kSumGroups; ++k) t += part[k][c];
+    float* out = col < hd ? dgq + col : dgk + (col - hd);
+    *out += t;
+  }
+}
+
+Turns turns_of(int hd, double theta) {
+  Turns t;
+  t.unit = 0.15915494309189533577;  // 1 / (2 pi)
+  double r = pow(theta, -2.0 / (double)hd);
+  for (int k = 0; k < 7; ++k, r *= r) t.ratio[k] = r;
+  return t;
+}
+
+// Warps that share a row's heads: one, unless there are too few rows to fill the GPU with one each.
+int warps_per_row_of(int rows, int heads, int slots, int sms) {
+  int w = 1;
+  while (w < kWarps && (long)rows * w < 16L * sms && w * slots < heads) w *= 2;
+  return w;
+}
+
+int sm_count() {
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+// Calls fn(lanes per head) with the smallest power of two that covers half / 8.
+template <class F>
+int with_lanes(int hd, F&& fn) {
+  const int need = hd / 16;
+  if (need <= 1) return fn(std::integral_constant<int, 1>{});
+  if (need <= 2) return fn(std::integral_constant<int, 2>{});
+  if (need <= 4) return fn(std::integral_constant<int, 4>{});
+  if (need <= 8) return fn(std::integral_constant<int, 8>{});
+  return fn(std::integral_constant<int, 16>{});
+}
+
+int grid_of(int rows, int rows_per_block, int sms) {
+  return (int)std::min<long>(((long)rows + rows_per_block - 1) / rows_per_block, 4L * sms);
+}
+
+}  // namespace
+
+int qk_norm_rope_blocks(int rows, int heads, int hd) {
+  int lanes = 1;
+  while (lanes * 16 < hd) lanes *= 2;
+  const int sms = sm_count();
+  return grid_of(rows, kWarps / warps_per_row_of(rows, heads, 32 / lanes, sms), sms);
+}
+
+int qk_norm_rope_fwd(const QkNormRopeArgs& a, cudaStream_t s) {
+  if (a.hd % 16 || a.hd < 16 || a.hd > 2 * kMaxHalf || a.S < 1) return -1;
+  if (a.rows == 0 || a.H + a.HK == 0) return 0;
+  const int sms = sm_count();
+  const Turns turns = turns_of(a.hd, a.theta);
+  return with_dtype(a.dtype, [&](auto v) {
+    using T = decltype(v);
+    return with_lanes(a.hd, [&](auto lanes) {
+      constexpr int G = decltype(lanes)::value;
+      const int w = warps_per_row_of(a.rows, a.H + a.HK, 32 / G, sms);
+      qk_norm_rope_fwd_kernel<T, G, sizeof(T) == 2 ? 2 : 1>
+          <<<grid_of(a.rows, kWarps / w, sms), kWarps * 32, 0, s>>>(
+              (const T*)a.x, a.ldx, (const T*)a.gq, (const T*)a.gk, (T*)a.out, a.ldo, a.rows, a.S, a.H, a.HK, a.hd,
+              a.eps, w, turns);
+      return (int)cudaGetLastError();
+    });
+  });
+}
+
+int qk_norm_rope_bwd(const QkNormRopeArgs& a, const void* dy, long lddy, float* partial, float* dgq, float* dgk,
+                     cudaStream_t s) {
+  if (a.hd % 16 || a.hd < 16 || a.hd > 2 * kMaxHalf || a.S < 1) return -1;
+  if (a.rows == 0 || a.H + a.HK == 0) return 0;
+  const int sms = sm_count();
+  const Turns turns = turns_of(a.hd, a.theta);
+  return with_dtype(a.dtype, [&](auto v) {
+    using T = decltype(v);
+    return with_lanes(a.hd, [&](auto lanes) {
+      constexpr int G = decltype(lanes)::value;
+      const int w = warps_per_row_of(a.rows, a.H + a.HK, 32 / G, sms);
+      const int blocks = grid_of(a.rows, kWarps / w, sms);
+      qk_norm_rope_bwd_kernel<T, G, 1><<<blocks, kWarps * 32, 0, s>>>(
+          (const T*)dy, lddy, (const T*)a.x, a.ldx, (const T*)a.gq, (const T*)a.gk, (T*)a.out, a.ldo, partial, a.rows,
+          a.S, a.H, a.HK, a.hd, a.eps, w, turns);
+      gain_sum_kernel<<<(2 * a.hd + kSumCols - 1) / kSumCols, kSumCols * kSumGroups, 0, s>>>(partial, blocks, a.hd,
+                                                                                             dgq, dgk);
+      return (int)cudaGetLastError();
+    });
+  });
+}
+
+}  // namespace mt

@@ -32,7 +32,7 @@ if os.environ.get("MT_ATTN_TRACE") == "1":
 SOURCES = [
     os.path.join(CSRC, f)
     for f in ("bindings.cpp", "gemm_tcgen05.cu", "norms.cu", "elementwise.cu", "cross_entropy.cu", "adam.cu",
-              "attention.cu")
+              "attention.cu", "qk_norm_rope.cu", "dropout.cu", "token_loss.cu")
     if os.path.exists(os.path.join(HERE, CSRC, f))
 ]
 
