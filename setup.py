@@ -29,6 +29,11 @@ NVCC_FLAGS = [
 if os.environ.get("MT_ATTN_TRACE") == "1":
     NVCC_FLAGS.append("-DMT_ATTN_TRACE")
 
+# Link the shared C++ runtime that torch itself uses.  A toolchain that only finds libstdc++.a would give
+# the module a copy of its own, and a refused argument would then crash in the unwinding or the message
+# formatting between the two instead of raising.
+LINK_FLAGS = ["-l:libstdc++.so.6"]
+
 SOURCES = [
     os.path.join(CSRC, f)
     for f in ("bindings.cpp", "gemm_tcgen05.cu", "norms.cu", "elementwise.cu", "cross_entropy.cu", "adam.cu",
@@ -42,6 +47,7 @@ EXTENSIONS = [
         sources=SOURCES,
         include_dirs=[os.path.join(HERE, CSRC)],
         extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": NVCC_FLAGS},
+        extra_link_args=LINK_FLAGS,
     )
 ]
 # Debug-checks build: MT_DEBUG_CHECKS=1 also builds meshtrain_b200.ops._C_debug, whose kernels check
@@ -54,6 +60,7 @@ if os.environ.get("MT_DEBUG_CHECKS") == "1":
         include_dirs=[os.path.join(HERE, CSRC)],
         extra_compile_args={"cxx": ["-O3", "-std=c++17", "-DMT_DEBUG_CHECKS"],
                             "nvcc": NVCC_FLAGS + ["-DMT_DEBUG_CHECKS"]},
+        extra_link_args=LINK_FLAGS,
     ))
 
 setup(
