@@ -134,10 +134,12 @@ _KERNEL_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _custom_float(t: torch.Tensor) -> bool:
-    """``_custom`` for the operators whose kernels also take fp16 and fp32."""
+    """``_custom`` for the operators whose kernels also take fp16 and fp32 (then ``_EXT`` is loaded).
+    Their bindings check the arguments themselves: a small call is bound by its launch."""
     if not (t.is_cuda and _BACKEND == "custom" and t.dtype in _KERNEL_DTYPES):
         return False
-    extension()
+    if _EXT is None:
+        extension()
     return True
 
 
@@ -173,10 +175,6 @@ def _mat(x: torch.Tensor) -> torch.Tensor:
     return buf[:, :cols]
 
 
-def _aligned(x: torch.Tensor) -> torch.Tensor:
-    """``x`` contiguous and starting on a 16-byte boundary (a copy where it is not)."""
-    x = x.contiguous()
-    return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
 # ----------------------------------------------------------------------------- linear
@@ -477,23 +475,17 @@ def _check_heads(name, qkv, q_gain, k_gain, seq_len, heads, kv_heads, head_dim, 
     for g, what in ((q_gain, "q_gain"), (k_gain, "k_gain")):
         _require(tuple(g.shape) == (head_dim,) and g.dtype == qkv.dtype and g.device == qkv.device,
                  f"{name}: {what} must be [head_dim] of qkv's dtype and device")
-    if _custom_float(qkv):
-        _require(head_dim % 16 == 0 and head_dim <= 256,
-                 f"{name}: head_dim {head_dim} unsupported by the kernel (multiples of 16 up to 256)")
     return (heads + kv_heads) * head_dim
 
 
 def _out_rows(name, out, like, rows, cols):
-    """``out`` checked as a row-major [rows, >= cols] matrix the kernels can write in place, or a new one."""
+    """``out`` checked as a row-major [rows, >= cols] matrix, or a new one as the kernels lay it out."""
     if out is None:
         ld = (cols + 7) // 8 * 8
         return torch.empty(rows, ld, dtype=like.dtype, device=like.device)[:, :cols]
-    ok = (out.dim() == 2 and out.shape[0] == rows and out.shape[1] >= cols and out.stride(1) == 1
-          and (rows < 2 or out.stride(0) >= cols) and out.dtype == like.dtype and out.device == like.device)
-    if _custom_float(like):
-        ok = ok and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0
-    _require(ok, f"{name}: out must be [rows, >= {cols}] row-major of the input's dtype and device, its rows on "
-                 "16-byte boundaries with a leading dimension that is a multiple of 8")
+    _require(out.dim() == 2 and out.shape[0] == rows and out.shape[1] >= cols and out.stride(1) == 1
+             and (rows < 2 or out.stride(0) >= cols) and out.dtype == like.dtype and out.device == like.device,
+             f"{name}: out must be [rows, >= {cols}] row-major of the input's dtype and device")
     return out[:, :cols]
 
 
@@ -518,13 +510,11 @@ def qk_norm_rope(qkv, q_gain, k_gain, seq_len: int, heads: int, kv_heads: int, h
     ``(mean(x^2) + eps)^-1/2`` times ``q_gain`` / ``k_gain`` [head_dim] and rotated as ``rope_`` does.
     Returns [T, (heads + kv_heads) * head_dim]; ``qkv`` itself is what the backward needs.
     """
+    if _custom_float(qkv):
+        return _EXT.qk_norm_rope_fwd(qkv, q_gain, k_gain, seq_len, heads, kv_heads, head_dim, theta, eps, out)
     cols = _check_heads("qk_norm_rope", qkv, q_gain, k_gain, seq_len, heads, kv_heads, head_dim, theta, eps)
     T = qkv.shape[0]
     res = _out_rows("qk_norm_rope", out, qkv, T, cols)
-    if _custom_float(qkv):
-        extension().qk_norm_rope_fwd(_mat(qkv), _aligned(q_gain), _aligned(k_gain), res, seq_len, heads, kv_heads, head_dim,
-                                     theta, eps)
-        return res
     dt, half = _acc(qkv), head_dim // 2
     x = qkv[:, :cols].to(dt).reshape(T, -1, head_dim)
     u = x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * _gain_rows(q_gain, k_gain, heads, kv_heads, dt)
@@ -544,6 +534,9 @@ def qk_norm_rope_bwd(dqk, qkv, q_gain, k_gain, seq_len: int, heads: int, kv_head
     itself (columns behind the heads stay as they are) or memory that does not overlap the inputs.
     Equal inputs give equal bits.
     """
+    if _custom_float(qkv):
+        return _EXT.qk_norm_rope_bwd(dqk, qkv, q_gain, k_gain, seq_len, heads, kv_heads, head_dim, theta, dq_gain,
+                                     dk_gain, eps, out)
     cols = _check_heads("qk_norm_rope_bwd", qkv, q_gain, k_gain, seq_len, heads, kv_heads, head_dim, theta, eps)
     T = qkv.shape[0]
     _require(dqk.dim() == 2 and dqk.shape[0] == T and dqk.shape[1] >= cols and dqk.dtype == qkv.dtype
@@ -552,10 +545,6 @@ def qk_norm_rope_bwd(dqk, qkv, q_gain, k_gain, seq_len: int, heads: int, kv_head
         _require(tuple(g.shape) == (head_dim,) and g.dtype == _acc(qkv) and g.device == qkv.device
                  and g.is_contiguous(), f"qk_norm_rope_bwd: {what} must be contiguous {_acc(qkv)} [head_dim]")
     res = _out_rows("qk_norm_rope_bwd", out, qkv, T, cols)
-    if _custom_float(qkv):
-        extension().qk_norm_rope_bwd(_mat(dqk), _mat(qkv), _aligned(q_gain), _aligned(k_gain), res, seq_len, heads, kv_heads,
-                                     head_dim, theta, eps, dq_gain, dk_gain)
-        return res
     dt, half = _acc(qkv), head_dim // 2
     x = qkv[:, :cols].to(dt).reshape(T, -1, head_dim)
     dy = dqk[:, :cols].to(dt).reshape(T, -1, head_dim)
@@ -616,28 +605,22 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset, residual: torch.Tensor
     draws another mask at each replay.  ``out`` may be ``x`` or ``residual``.  Dropped elements add
     exactly 0, whatever ``x`` holds there.
     """
-    _require(0.0 <= p < 1.0 and round(p * 65536) < 65536, f"dropout: p must be in [0, 1) and round below 1, got {p}")
-    cut = round(p * 65536)
-    _require(0 <= seed < 1 << 64, "dropout: seed must be a 64-bit unsigned integer")
+    cut = round(p * 65536) if 0.0 <= p < 1.0 else 65536
+    _require(cut < 65536, f"dropout: p must be in [0, 1) and round below 1, got {p}")
     on_device = isinstance(offset, torch.Tensor)
-    if on_device:
-        _require(offset.numel() == 1 and offset.dtype == torch.int64 and offset.device == x.device,
-                 "dropout: an offset tensor must be one int64 on x's device")
-        offset = offset.reshape(1)
-    else:
-        _require(0 <= offset < 1 << 64, "dropout: offset must be a 64-bit unsigned integer")
+    _require(0 <= seed < 1 << 64 and (on_device or 0 <= offset < 1 << 64),
+             "dropout: seed and offset must be 64-bit unsigned integers")
+    if _custom_float(x):
+        return _EXT.dropout(x, cut, _signed64(seed), 0 if on_device else _signed64(offset),
+                            offset if on_device else None, residual, out)
+    _require(not on_device or (offset.numel() == 1 and offset.dtype == torch.int64 and offset.device == x.device),
+             "dropout: an offset tensor must be one int64 on x's device")
     for t, what in ((residual, "residual"), (out, "out")):
         _require(t is None or (t.shape == x.shape and t.dtype == x.dtype and t.device == x.device),
                  f"dropout: {what} must have x's shape, dtype and device")
     _require(out is None or out.is_contiguous(), "dropout: out must be contiguous")
-    if _custom_float(x):
-        _require(out is None or out.data_ptr() % 16 == 0, "dropout: out must start on a 16-byte boundary")
-        res = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-        extension().dropout(_aligned(x), None if residual is None else _aligned(residual), res, cut,
-                            _signed64(seed), 0 if on_device else _signed64(offset), offset if on_device else None)
-        return res
     dt = _acc(x)
-    keep = _keep_mask(x.shape, cut, seed, offset, x.device)
+    keep = _keep_mask(x.shape, cut, seed, offset.reshape(()) if on_device else offset, x.device)
     y = torch.where(keep, x.to(dt) * (65536 / (65536 - cut)), 0.0)
     if residual is not None:
         y = residual.to(dt) + y
@@ -690,11 +673,6 @@ def _check_logits(name, logits, vocab, targets):
     return _vector(targets, logits.shape[0], logits, torch.int64, f"{name}: targets")
 
 
-def _rows_of(logits, vocab):
-    """The first ``vocab`` columns for the kernels; rows of narrower layouts are copied into padded ones."""
-    return _mat(logits[:, :vocab])
-
-
 def _plain_logprobs(logits, vocab, tg):
     dt = _acc(logits)
     lg = logits[:, :vocab].to(dt)
@@ -724,9 +702,9 @@ def token_logprobs(logits: torch.Tensor, vocab: int, targets: torch.Tensor):
     ``logits`` [T, >= vocab] as the LM head's GEMM leaves them.  A target outside [0, vocab) marks a row
     without a token: logp 0.  A row whose logits are all -inf has m = logp = -inf and the sum 0.
     """
-    tg = _check_logits("token_logprobs", logits, vocab, targets)
     if _custom_float(logits):
-        return tuple(extension().token_logprobs(_rows_of(logits, vocab), vocab, tg))
+        return _EXT.token_logprobs(logits, vocab, targets)
+    tg = _check_logits("token_logprobs", logits, vocab, targets)
     return _plain_logprobs(logits, vocab, tg)
 
 
@@ -739,14 +717,13 @@ def token_logprobs_bwd(logits: torch.Tensor, vocab: int, targets: torch.Tensor, 
     hold.  ``out`` may be ``logits`` (overwritten); otherwise a new matrix, whose rows are padded
     to a multiple of 8 columns as the LM head's GEMMs take them.  Returns its first ``vocab`` columns.
     """
+    if _custom_float(logits):
+        return _EXT.token_logprobs_bwd(logits, vocab, targets, stats, dlogps, out)
     tg = _check_logits("token_logprobs_bwd", logits, vocab, targets)
     T, dt = logits.shape[0], _acc(logits)
     stats = _vector(stats, 2 * T, logits, dt, "token_logprobs_bwd: stats")
     dlogps = _vector(dlogps, T, logits, dt, "token_logprobs_bwd: dlogps")
     res = _out_rows("token_logprobs_bwd", out, logits, T, vocab)
-    if _custom_float(logits):
-        extension().token_logprobs_bwd(_rows_of(logits, vocab), vocab, tg, _aligned(stats), dlogps, res)
-        return res
     return _plain_dlogits(logits, vocab, tg, stats, dlogps, res)
 
 
@@ -767,6 +744,9 @@ def policy_loss_chunk(logits: torch.Tensor, vocab: int, targets: torch.Tensor, o
     logps [T], dlogits), the last the gradient of ``grad_scale * sum(losses)``; ``out`` as in
     ``token_logprobs_bwd``.  All per-row tensors are fp32 [T].
     """
+    if _custom_float(logits):
+        return _EXT.policy_loss(logits, vocab, targets, old_logps, advantages, weights, ref_logps, clip_low, clip_high,
+                                kl_coef, grad_scale, out)
     name = "policy_loss_chunk"
     tg = _check_logits(name, logits, vocab, targets)
     T, dt = logits.shape[0], _acc(logits)
@@ -777,10 +757,6 @@ def policy_loss_chunk(logits: torch.Tensor, vocab: int, targets: torch.Tensor, o
     if kl_coef == 0.0:
         ref = None
     res = _out_rows(name, out, logits, T, vocab)
-    if _custom_float(logits):
-        losses, logps = extension().policy_loss(_rows_of(logits, vocab), vocab, tg, old, ref, adv, w, clip_low,
-                                                clip_high, kl_coef, grad_scale, res)
-        return losses, logps, res
     lp, stats = _plain_logprobs(logits, vocab, tg)
     valid = (tg >= 0) & (tg < vocab)
     lpd = lp.double()
@@ -814,18 +790,17 @@ def preference_loss(logps: torch.Tensor, ref_logps: torch.Tensor, mask: torch.Te
     An empty row has r = 0 and no gradient.  Returns (losses [P], rewards [2 P] = beta r, dlogps [2 P, S],
     the gradient of ``grad_scale * sum(losses)``).  Masked tokens are not looked at.
     """
+    _require(form in ("sigmoid", "squared"), f"preference_loss: unknown form {form!r} (sigmoid, squared)")
+    if _custom_float(logps):
+        return _EXT.preference_loss(logps, ref_logps, mask, beta, label_smoothing, form == "squared", grad_scale)
     dt = _acc(logps)
     _require(logps.dim() == 2 and logps.shape[0] % 2 == 0 and logps.dtype == dt,
              "preference_loss: logps must be fp32 [2 pairs, S]")
-    _require(form in ("sigmoid", "squared"), f"preference_loss: unknown form {form!r} (sigmoid, squared)")
     _require(beta > 0 and 0.0 <= label_smoothing <= 1.0, "preference_loss: needs beta > 0 and 0 <= label_smoothing <= 1")
     _require(form == "sigmoid" or label_smoothing == 0.0, "preference_loss: label_smoothing is the sigmoid form's")
     for t, n, want in ((ref_logps, "ref_logps", dt), (mask, "mask", torch.bool)):
         _require(t.shape == logps.shape and t.dtype == want and t.device == logps.device,
                  f"preference_loss: {n} must be {want} with logps's shape and device")
-    if _custom_float(logps):
-        return tuple(extension().preference_loss(logps.contiguous(), ref_logps.contiguous(), mask.contiguous(), beta,
-                                                 label_smoothing, form == "squared", grad_scale))
     r = torch.where(mask, logps.double() - ref_logps, 0.0).sum(-1)
     r0, r1 = r[0::2], r[1::2]
     if form == "sigmoid":

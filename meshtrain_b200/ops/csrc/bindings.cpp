@@ -247,178 +247,233 @@ void cross_entropy_(Tensor logits, int64_t V, Tensor targets, Tensor loss_sum, d
                   "cross_entropy");
 }
 
+// The functions below refuse bad arguments with a ValueError and take any layout: what the kernels
+// cannot read in place is copied first.
+
 // Element type code of mt_api.h.
 int dtype_code(const Tensor& t, const char* name) {
   switch (t.scalar_type()) {
     case at::kBFloat16: return 0;
     case at::kHalf: return 1;
     case at::kFloat: return 2;
-    default: TORCH_CHECK(false, name, " has dtype ", t.scalar_type(), ", expected bfloat16, float16 or float32");
+    default: TORCH_CHECK_VALUE(false, name, " has dtype ", t.scalar_type(), ", expected bfloat16, float16 or float32");
   }
   return -1;
 }
-// A row-major matrix whose rows start on 16-byte boundaries, on `like`'s device and of its type.
-void check_rows_like(const Tensor& t, const char* name, const Tensor& like, int64_t rows, int64_t cols) {
-  TORCH_CHECK(t.is_cuda() && t.get_device() == like.get_device(), name, " must be on ", like.device());
-  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " has dtype ", t.scalar_type(), ", expected ",
-              like.scalar_type());
-  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) >= cols && t.stride(1) == 1, name, " must be [", rows,
-              ", >= ", cols, "] row-major");
-  TORCH_CHECK(rows < 2 || t.stride(0) >= cols, name, " rows overlap");
-  TORCH_CHECK(rows < INT32_MAX && cols < INT32_MAX, name, " is too large");
-  TORCH_CHECK(t.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0, name,
-              " rows must be 16-byte aligned with a leading dimension that is a multiple of 8");
+bool aligned16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+// Rows the kernels read and write in place: unit column stride, 16-byte aligned, a leading dimension
+// that is a multiple of 8.
+bool is_rows(const Tensor& t) {
+  return t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && aligned16(t);
+}
+Tensor padded_rows(const Tensor& like, int64_t rows, int64_t cols) {
+  const int64_t ld = (cols + 7) / 8 * 8;
+  Tensor t = torch::empty({rows, ld}, like.options());
+  return ld == cols ? t : t.narrow(1, 0, cols);
+}
+// The first `cols` columns of a matrix of at least that many, on `like`'s device and of its type, as rows.
+Tensor as_rows(const Tensor& t, const char* name, const Tensor& like, int64_t rows, int64_t cols) {
+  TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == rows && t.size(1) >= cols && t.scalar_type() == like.scalar_type() &&
+                        t.device() == like.device(),
+                    name, " must be [", rows, ", >= ", cols, "] ", like.scalar_type(), " on ", like.device());
+  TORCH_CHECK_VALUE(rows < INT32_MAX && cols < INT32_MAX, name, " is too large");
+  if (is_rows(t)) return t;
+  Tensor copy = padded_rows(like, rows, cols);
+  copy.copy_(t.narrow(1, 0, cols));
+  return copy;
+}
+// `out` checked for in-place writing, or new rows.
+Tensor out_rows(const c10::optional<Tensor>& out, const char* name, const Tensor& like, int64_t rows, int64_t cols) {
+  if (!out) return padded_rows(like, rows, cols);
+  TORCH_CHECK_VALUE(out->dim() == 2 && out->size(0) == rows && out->size(1) >= cols &&
+                        out->scalar_type() == like.scalar_type() && out->device() == like.device() &&
+                        out->stride(1) == 1 && out->stride(0) % 8 == 0 && (rows < 2 || out->stride(0) >= cols) &&
+                        aligned16(*out),
+                    name, ": out must be [rows, >= ", cols, "] row-major of the input's dtype and device, its rows on ",
+                    "16-byte boundaries with a leading dimension that is a multiple of 8");
+  return out->size(1) == cols ? *out : out->narrow(1, 0, cols);
 }
 // A contiguous vector of n values on `like`'s device.
-void check_vector(const Tensor& t, const char* name, at::ScalarType dt, const Tensor& like, int64_t n) {
-  check_cuda(t, name, dt);
-  TORCH_CHECK(t.get_device() == like.get_device(), name, " must be on ", like.device());
-  TORCH_CHECK(t.is_contiguous() && t.numel() == n, name, " must be contiguous with ", n, " values");
+Tensor as_vector(const Tensor& t, const char* name, at::ScalarType dt, const Tensor& like, int64_t n) {
+  TORCH_CHECK_VALUE(t.numel() == n && t.scalar_type() == dt && t.device() == like.device(), name, " must have ", n,
+                    " values of ", dt, " on ", like.device(), ", got ", t.sizes(), " of ", t.scalar_type(), " on ",
+                    t.device());
+  return t.contiguous();
+}
+Tensor as_aligned(const Tensor& t) {
+  Tensor c = t.contiguous();
+  return aligned16(c) ? c : c.clone();
 }
 
-mt::QkNormRopeArgs qk_args(const Tensor& x, const Tensor& gq, const Tensor& gk, const Tensor& out, int64_t S, int64_t H,
-                           int64_t HK, int64_t hd, double theta, double eps) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2, "qk_norm_rope: qkv must be a CUDA matrix");
-  const int code = dtype_code(x, "qkv");
-  TORCH_CHECK(hd % 16 == 0 && hd >= 16 && hd <= 256, "qk_norm_rope: head_dim ", hd,
-              " unsupported (multiples of 16 up to 256)");
-  TORCH_CHECK(H >= 0 && HK >= 0 && H + HK >= 1 && H + HK <= 65536 && S >= 1 && S < INT32_MAX,
-              "qk_norm_rope: bad heads or seq_len");
-  TORCH_CHECK(theta > 0 && eps >= 0, "qk_norm_rope: theta must be positive and eps not negative");
-  const int64_t rows = x.size(0), cols = (H + HK) * hd;
-  check_rows_like(x, "qkv", x, rows, cols);
-  check_rows_like(out, "out", x, rows, cols);
-  check_vector(gq, "q_gain", x.scalar_type(), x, hd);
-  check_vector(gk, "k_gain", x.scalar_type(), x, hd);
-  TORCH_CHECK((reinterpret_cast<uintptr_t>(gq.data_ptr()) & 15) == 0 &&
-                  (reinterpret_cast<uintptr_t>(gk.data_ptr()) & 15) == 0,
-              "qk_norm_rope: gains must be 16-byte aligned");
+struct QkInputs {
   mt::QkNormRopeArgs a{};
-  a.x = x.data_ptr();
-  a.ldx = x.stride(0);
-  a.gq = gq.data_ptr();
-  a.gk = gk.data_ptr();
-  a.out = out.data_ptr();
-  a.ldo = out.stride(0);
-  a.dtype = code;
-  a.rows = (int)rows;
-  a.S = (int)S;
-  a.H = (int)H;
-  a.HK = (int)HK;
-  a.hd = (int)hd;
-  a.eps = (float)eps;
-  a.theta = theta;
-  return a;
+  Tensor x, gq, gk, out;  // keep copies alive
+};
+void qk_inputs(QkInputs& in, const char* name, const Tensor& qkv, const Tensor& gq, const Tensor& gk,
+                   const c10::optional<Tensor>& out, int64_t S, int64_t H, int64_t HK, int64_t hd, double theta,
+                   double eps) {
+  TORCH_CHECK_VALUE(qkv.is_cuda() && qkv.dim() == 2 && H >= 0 && HK >= 0 && H + HK >= 1 && H + HK <= 65536 && hd >= 2,
+                    name, ": qkv must be [rows, >= (heads + kv_heads) * head_dim]");
+  TORCH_CHECK_VALUE(hd % 16 == 0 && hd <= 256, name, ": head_dim ", hd,
+                    " unsupported by the kernel (multiples of 16 up to 256)");
+  TORCH_CHECK_VALUE(S >= 1 && S < INT32_MAX && theta > 0 && eps >= 0, name,
+                    ": needs seq_len >= 1, theta > 0 and eps >= 0");
+  in.a.dtype = dtype_code(qkv, name);
+  const int64_t rows = qkv.size(0), cols = (H + HK) * hd;
+  for (auto* g : {&gq, &gk})
+    TORCH_CHECK_VALUE(g->dim() == 1 && g->size(0) == hd && g->scalar_type() == qkv.scalar_type() &&
+                          g->device() == qkv.device(),
+                      name, ": gains must be [head_dim] of qkv's dtype and device");
+  in.x = as_rows(qkv, name, qkv, rows, cols);
+  in.out = out_rows(out, name, qkv, rows, cols);
+  in.gq = as_aligned(gq);
+  in.gk = as_aligned(gk);
+  in.a.x = in.x.data_ptr();
+  in.a.ldx = in.x.stride(0);
+  in.a.gq = in.gq.data_ptr();
+  in.a.gk = in.gk.data_ptr();
+  in.a.out = in.out.data_ptr();
+  in.a.ldo = in.out.stride(0);
+  in.a.rows = (int)rows;
+  in.a.S = (int)S;
+  in.a.H = (int)H;
+  in.a.HK = (int)HK;
+  in.a.hd = (int)hd;
+  in.a.eps = (float)eps;
+  in.a.theta = theta;
 }
 
-void qk_norm_rope_fwd(Tensor x, Tensor gq, Tensor gk, Tensor out, int64_t S, int64_t H, int64_t HK, int64_t hd,
-                      double theta, double eps) {
-  const mt::QkNormRopeArgs a = qk_args(x, gq, gk, out, S, H, HK, hd, theta, eps);
-  c10::cuda::CUDAGuard guard(x.get_device());
-  MT_CHECK_LAUNCH(mt::qk_norm_rope_fwd(a, stream_of(x)), "qk_norm_rope");
+Tensor qk_norm_rope_fwd(const Tensor& qkv, const Tensor& gq, const Tensor& gk, int64_t S, int64_t H, int64_t HK,
+                        int64_t hd, double theta, double eps, const c10::optional<Tensor>& out) {
+  c10::cuda::OptionalCUDAGuard guard(at::device_of(qkv));
+  QkInputs in;
+  qk_inputs(in, "qk_norm_rope", qkv, gq, gk, out, S, H, HK, hd, theta, eps);
+  MT_CHECK_LAUNCH(mt::qk_norm_rope_fwd(in.a, stream_of(qkv)), "qk_norm_rope");
+  return in.out;
 }
 
-void qk_norm_rope_bwd(Tensor dy, Tensor x, Tensor gq, Tensor gk, Tensor out, int64_t S, int64_t H, int64_t HK,
-                      int64_t hd, double theta, double eps, Tensor dgq, Tensor dgk) {
-  const mt::QkNormRopeArgs a = qk_args(x, gq, gk, out, S, H, HK, hd, theta, eps);
-  check_rows_like(dy, "dqk", x, x.size(0), (H + HK) * hd);
-  check_vector(dgq, "dq_gain", at::kFloat, x, hd);
-  check_vector(dgk, "dk_gain", at::kFloat, x, hd);
-  if (a.rows == 0) return;
-  c10::cuda::CUDAGuard guard(x.get_device());
-  auto partial = torch::empty({mt::qk_norm_rope_blocks(a.rows, a.H + a.HK, a.hd), 2 * hd},
-                              x.options().dtype(at::kFloat));
-  MT_CHECK_LAUNCH(mt::qk_norm_rope_bwd(a, dy.data_ptr(), dy.stride(0), partial.data_ptr<float>(),
-                                       dgq.data_ptr<float>(), dgk.data_ptr<float>(), stream_of(x)),
+Tensor qk_norm_rope_bwd(const Tensor& dqk, const Tensor& qkv, const Tensor& gq, const Tensor& gk, int64_t S, int64_t H,
+                        int64_t HK, int64_t hd, double theta, Tensor dgq, Tensor dgk, double eps,
+                        const c10::optional<Tensor>& out) {
+  c10::cuda::OptionalCUDAGuard guard(at::device_of(qkv));
+  QkInputs in;
+  qk_inputs(in, "qk_norm_rope_bwd", qkv, gq, gk, out, S, H, HK, hd, theta, eps);
+  const Tensor dy = as_rows(dqk, "qk_norm_rope_bwd: dqk", qkv, qkv.size(0), (H + HK) * hd);
+  for (auto* g : {&dgq, &dgk})
+    TORCH_CHECK_VALUE(g->dim() == 1 && g->size(0) == hd && g->scalar_type() == at::kFloat &&
+                          g->device() == qkv.device() && g->is_contiguous(),
+                      "qk_norm_rope_bwd: dq_gain and dk_gain must be contiguous float32 [head_dim]");
+  if (in.a.rows == 0) return in.out;
+  auto partial = torch::empty({mt::qk_norm_rope_blocks(in.a.rows, in.a.H + in.a.HK, in.a.hd), 2 * hd}, dgq.options());
+  MT_CHECK_LAUNCH(mt::qk_norm_rope_bwd(in.a, dy.data_ptr(), dy.stride(0), partial.data_ptr<float>(),
+                                       dgq.data_ptr<float>(), dgk.data_ptr<float>(), stream_of(qkv)),
                   "qk_norm_rope_bwd");
+  return in.out;
 }
 
-// seed and offset carry 64 unsigned bits in int64.
-void dropout(Tensor x, c10::optional<Tensor> residual, Tensor out, int64_t cut, int64_t seed, int64_t offset,
-             c10::optional<Tensor> offset_tensor) {
-  TORCH_CHECK(x.is_cuda(), "dropout: x must be a CUDA tensor");
+// seed carries 64 unsigned bits in int64, and so does an offset that is no tensor.
+Tensor dropout(const Tensor& x, int64_t cut, int64_t seed, int64_t offset, const c10::optional<Tensor>& offset_tensor,
+               const c10::optional<Tensor>& residual, const c10::optional<Tensor>& out) {
+  TORCH_CHECK_VALUE(x.is_cuda(), "dropout: x must be a CUDA tensor");
+  TORCH_CHECK_VALUE(cut >= 0 && cut < 65536, "dropout: p must be in [0, 1) and round below 1");
+  c10::cuda::OptionalCUDAGuard guard(at::device_of(x));
   mt::DropoutArgs a{};
   a.dtype = dtype_code(x, "x");
-  check_rows(x, "x");
-  a.x = x.data_ptr();
+  for (auto* t : {&residual, &out})
+    TORCH_CHECK_VALUE(!*t || ((*t)->sizes() == x.sizes() && (*t)->scalar_type() == x.scalar_type() &&
+                              (*t)->device() == x.device()),
+                      "dropout: residual and out must have x's shape, dtype and device");
+  TORCH_CHECK_VALUE(!out || (out->is_contiguous() && aligned16(*out)),
+                    "dropout: out must be contiguous and start on a 16-byte boundary");
+  const Tensor xc = as_aligned(x);
+  Tensor rc, res = out ? *out : torch::empty(x.sizes(), x.options());
+  a.x = xc.data_ptr();
   a.n = x.numel();
-  for (auto* t : {residual ? &*residual : &x, &out}) {
-    TORCH_CHECK(t->is_cuda() && t->get_device() == x.get_device() && t->scalar_type() == x.scalar_type() &&
-                    t->numel() == x.numel(),
-                "dropout: residual and out must have x's device, dtype and size");
-    check_rows(*t, "dropout: residual and out");
+  if (residual) {
+    rc = as_aligned(*residual);
+    a.residual = rc.data_ptr();
   }
-  if (residual) a.residual = residual->data_ptr();
-  a.out = out.data_ptr();
-  TORCH_CHECK(cut >= 0 && cut < 65536, "dropout: p must round to less than 1");
+  a.out = res.data_ptr();
   a.cut = (uint32_t)cut;
   a.seed = (uint64_t)seed;
   a.offset = (uint64_t)offset;
   if (offset_tensor) {
-    check_vector(*offset_tensor, "offset", at::kLong, x, 1);
+    TORCH_CHECK_VALUE(offset_tensor->numel() == 1 && offset_tensor->scalar_type() == at::kLong &&
+                          offset_tensor->device() == x.device(),
+                      "dropout: an offset tensor must be one int64 on x's device");
     a.offset_ptr = offset_tensor->data_ptr<int64_t>();
   }
-  c10::cuda::CUDAGuard guard(x.get_device());
   MT_CHECK_LAUNCH(mt::dropout_apply(a, stream_of(x)), "dropout");
+  return res;
 }
 
-void check_logits(const Tensor& logits, int64_t V, const Tensor& targets) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && V >= 1, "logits must be a CUDA matrix [rows, >= vocab]");
-  check_rows_like(logits, "logits", logits, logits.size(0), V);
-  check_vector(targets, "targets", at::kLong, logits, logits.size(0));
+Tensor as_logits(const char* name, const Tensor& logits, int64_t V) {
+  TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 && V >= 1 && logits.size(1) >= V, name,
+                    ": logits must be [rows, >= vocab]");
+  return as_rows(logits, name, logits, logits.size(0), V);
 }
 
-std::vector<Tensor> token_logprobs(Tensor logits, int64_t V, Tensor targets) {
-  check_logits(logits, V, targets);
+std::tuple<Tensor, Tensor> token_logprobs(const Tensor& logits, int64_t V, const Tensor& targets) {
+  c10::cuda::OptionalCUDAGuard guard(at::device_of(logits));
+  const Tensor x = as_logits("token_logprobs", logits, V);
   const int64_t rows = logits.size(0);
-  c10::cuda::CUDAGuard guard(logits.get_device());
+  const Tensor t = as_vector(targets, "token_logprobs: targets", at::kLong, logits, rows);
   auto fopts = logits.options().dtype(at::kFloat);
   auto logps = torch::empty({rows}, fopts), stats = torch::empty({rows, 2}, fopts);
-  MT_CHECK_LAUNCH(mt::token_logprobs(logits.data_ptr(), logits.stride(0), dtype_code(logits, "logits"),
-                                     targets.data_ptr<int64_t>(), logps.data_ptr<float>(), stats.data_ptr<float>(),
-                                     (int)rows, (int)V, stream_of(logits)),
+  MT_CHECK_LAUNCH(mt::token_logprobs(x.data_ptr(), x.stride(0), dtype_code(logits, "logits"), t.data_ptr<int64_t>(),
+                                     logps.data_ptr<float>(), stats.data_ptr<float>(), (int)rows, (int)V,
+                                     stream_of(logits)),
                   "token_logprobs");
   return {logps, stats};
 }
 
-void token_logprobs_bwd(Tensor logits, int64_t V, Tensor targets, Tensor stats, Tensor dlogps, Tensor out) {
-  check_logits(logits, V, targets);
+Tensor token_logprobs_bwd(const Tensor& logits, int64_t V, const Tensor& targets, const Tensor& stats,
+                          const Tensor& dlogps, const c10::optional<Tensor>& out) {
+  c10::cuda::OptionalCUDAGuard guard(at::device_of(logits));
+  const Tensor x = as_logits("token_logprobs_bwd", logits, V);
   const int64_t rows = logits.size(0);
-  check_vector(stats, "stats", at::kFloat, logits, 2 * rows);
-  TORCH_CHECK((reinterpret_cast<uintptr_t>(stats.data_ptr()) & 7) == 0, "stats must be 8-byte aligned");
-  check_vector(dlogps, "dlogps", at::kFloat, logits, rows);
-  check_rows_like(out, "out", logits, rows, V);
-  c10::cuda::CUDAGuard guard(logits.get_device());
-  MT_CHECK_LAUNCH(mt::token_logprobs_bwd(logits.data_ptr(), logits.stride(0), dtype_code(logits, "logits"),
-                                         targets.data_ptr<int64_t>(), stats.data_ptr<float>(),
-                                         dlogps.data_ptr<float>(), out.data_ptr(), out.stride(0), (int)rows, (int)V,
-                                         stream_of(logits)),
+  const Tensor t = as_vector(targets, "token_logprobs_bwd: targets", at::kLong, logits, rows);
+  const Tensor st = as_aligned(as_vector(stats, "token_logprobs_bwd: stats", at::kFloat, logits, 2 * rows));
+  const Tensor up = as_vector(dlogps, "token_logprobs_bwd: dlogps", at::kFloat, logits, rows);
+  Tensor res = out_rows(out, "token_logprobs_bwd", logits, rows, V);
+  MT_CHECK_LAUNCH(mt::token_logprobs_bwd(x.data_ptr(), x.stride(0), dtype_code(logits, "logits"), t.data_ptr<int64_t>(),
+                                         st.data_ptr<float>(), up.data_ptr<float>(), res.data_ptr(), res.stride(0),
+                                         (int)rows, (int)V, stream_of(logits)),
                   "token_logprobs_bwd");
+  return res;
 }
 
-std::vector<Tensor> policy_loss(Tensor logits, int64_t V, Tensor targets, Tensor old_logps,
-                                c10::optional<Tensor> ref_logps, Tensor advantages, c10::optional<Tensor> weights,
-                                double clip_low, double clip_high, double kl_coef, double grad_scale, Tensor out) {
-  check_logits(logits, V, targets);
+std::tuple<Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, int64_t V, const Tensor& targets,
+                                               const Tensor& old_logps, const Tensor& advantages,
+                                               const c10::optional<Tensor>& weights,
+                                               const c10::optional<Tensor>& ref_logps, double clip_low,
+                                               double clip_high, double kl_coef, double grad_scale,
+                                               const c10::optional<Tensor>& out) {
+  c10::cuda::OptionalCUDAGuard guard(at::device_of(logits));
+  const Tensor x = as_logits("policy_loss_chunk", logits, V);
   const int64_t rows = logits.size(0);
-  check_vector(old_logps, "old_logps", at::kFloat, logits, rows);
-  check_vector(advantages, "advantages", at::kFloat, logits, rows);
-  if (ref_logps) check_vector(*ref_logps, "ref_logps", at::kFloat, logits, rows);
-  if (weights) check_vector(*weights, "weights", at::kFloat, logits, rows);
-  check_rows_like(out, "out", logits, rows, V);
-  c10::cuda::CUDAGuard guard(logits.get_device());
+  TORCH_CHECK_VALUE(clip_low >= 0 && clip_low <= 1 && clip_high >= 0,
+                    "policy_loss_chunk: needs 0 <= clip_low <= 1 and clip_high >= 0");
+  TORCH_CHECK_VALUE(kl_coef == 0 || ref_logps, "policy_loss_chunk: a KL term needs ref_logps");
+  const Tensor t = as_vector(targets, "policy_loss_chunk: targets", at::kLong, logits, rows);
+  const Tensor old = as_vector(old_logps, "policy_loss_chunk: old_logps", at::kFloat, logits, rows);
+  const Tensor adv = as_vector(advantages, "policy_loss_chunk: advantages", at::kFloat, logits, rows);
+  Tensor w, ref;
+  if (weights) w = as_vector(*weights, "policy_loss_chunk: weights", at::kFloat, logits, rows);
+  if (ref_logps) ref = as_vector(*ref_logps, "policy_loss_chunk: ref_logps", at::kFloat, logits, rows);
+  Tensor res = out_rows(out, "policy_loss_chunk", logits, rows, V);
   auto losses = torch::empty({rows}, logits.options().dtype(at::kFloat)), logps = torch::empty_like(losses);
   mt::PolicyArgs a{};
-  a.logits = logits.data_ptr();
-  a.ld = logits.stride(0);
-  a.out = out.data_ptr();
-  a.ldo = out.stride(0);
+  a.logits = x.data_ptr();
+  a.ld = x.stride(0);
+  a.out = res.data_ptr();
+  a.ldo = res.stride(0);
   a.dtype = dtype_code(logits, "logits");
-  a.targets = targets.data_ptr<int64_t>();
-  a.old_logps = old_logps.data_ptr<float>();
-  a.ref_logps = ref_logps ? ref_logps->data_ptr<float>() : nullptr;
-  a.advantages = advantages.data_ptr<float>();
-  a.weights = weights ? weights->data_ptr<float>() : nullptr;
+  a.targets = t.data_ptr<int64_t>();
+  a.old_logps = old.data_ptr<float>();
+  a.ref_logps = kl_coef != 0 ? ref.data_ptr<float>() : nullptr;
+  a.advantages = adv.data_ptr<float>();
+  a.weights = weights ? w.data_ptr<float>() : nullptr;
   a.losses = losses.data_ptr<float>();
   a.logps = logps.data_ptr<float>();
   a.rows = (int)rows;
@@ -427,26 +482,32 @@ std::vector<Tensor> policy_loss(Tensor logits, int64_t V, Tensor targets, Tensor
   a.clip_high = clip_high;
   a.kl_coef = kl_coef;
   a.grad_scale = grad_scale;
-  MT_CHECK_LAUNCH(mt::policy_loss(a, stream_of(logits)), "policy_loss");
-  return {losses, logps};
+  MT_CHECK_LAUNCH(mt::policy_loss(a, stream_of(logits)), "policy_loss_chunk");
+  return {losses, logps, res};
 }
 
-std::vector<Tensor> preference_loss(Tensor logps, Tensor ref_logps, Tensor mask, double beta, double label_smoothing,
-                                    bool squared, double grad_scale) {
-  check_cuda(logps, "logps", at::kFloat);
-  TORCH_CHECK(logps.dim() == 2 && logps.size(0) % 2 == 0 && logps.size(1) < INT32_MAX && logps.is_contiguous(),
-              "preference_loss: logps must be contiguous [2 pairs, S]");
-  check_vector(ref_logps, "ref_logps", at::kFloat, logps, logps.numel());
-  check_vector(mask, "mask", at::kBool, logps, logps.numel());
+std::tuple<Tensor, Tensor, Tensor> preference_loss(const Tensor& logps, const Tensor& ref_logps, const Tensor& mask,
+                                                   double beta, double label_smoothing, bool squared,
+                                                   double grad_scale) {
+  TORCH_CHECK_VALUE(logps.is_cuda() && logps.dim() == 2 && logps.size(0) % 2 == 0 &&
+                        logps.scalar_type() == at::kFloat && logps.size(1) < INT32_MAX && logps.size(0) < INT32_MAX,
+                    "preference_loss: logps must be fp32 [2 pairs, S]");
+  TORCH_CHECK_VALUE(beta > 0 && label_smoothing >= 0 && label_smoothing <= 1,
+                    "preference_loss: needs beta > 0 and 0 <= label_smoothing <= 1");
+  TORCH_CHECK_VALUE(!squared || label_smoothing == 0, "preference_loss: label_smoothing is the sigmoid form's");
+  TORCH_CHECK_VALUE(ref_logps.sizes() == logps.sizes() && mask.sizes() == logps.sizes(),
+                    "preference_loss: ref_logps and mask must have logps's shape");
+  c10::cuda::OptionalCUDAGuard guard(at::device_of(logps));
   const int64_t pairs = logps.size(0) / 2;
-  TORCH_CHECK(pairs < INT32_MAX, "preference_loss: too many pairs");
-  c10::cuda::CUDAGuard guard(logps.get_device());
+  const Tensor lp = logps.contiguous();
+  const Tensor ref = as_vector(ref_logps, "preference_loss: ref_logps", at::kFloat, logps, logps.numel());
+  const Tensor m = as_vector(mask, "preference_loss: mask", at::kBool, logps, logps.numel());
   auto losses = torch::empty({pairs}, logps.options()), rewards = torch::empty({2 * pairs}, logps.options());
-  auto dlogps = torch::empty_like(logps);
+  auto dlogps = torch::empty(logps.sizes(), logps.options());
   mt::PreferenceArgs a{};
-  a.logps = logps.data_ptr<float>();
-  a.ref_logps = ref_logps.data_ptr<float>();
-  a.mask = reinterpret_cast<const uint8_t*>(mask.data_ptr<bool>());
+  a.logps = lp.data_ptr<float>();
+  a.ref_logps = ref.data_ptr<float>();
+  a.mask = reinterpret_cast<const uint8_t*>(m.data_ptr<bool>());
   a.losses = losses.data_ptr<float>();
   a.rewards = rewards.data_ptr<float>();
   a.dlogps = dlogps.data_ptr<float>();
