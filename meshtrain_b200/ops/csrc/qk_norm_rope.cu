@@ -14,11 +14,20 @@
 // is spread over G lanes, each holding 8 adjacent values of either half, so that the rotation's pairs
 // meet in one thread, every access is a 16-byte vector and a norm is log2(G) shuffles.  A warp takes
 // one row (or a share of its heads when there are few rows) and computes the row's sines once for
-// all heads.
+// all heads.  The backward sweeps the query heads of its rows, then the key heads, so that a thread
+// holds one gain and one gain gradient, and what it will read is on its way three turns ahead, by
+// asynchronous copies into slots of shared memory that no other thread touches: with plain loads,
+// registers limited what was in flight (115 us instead of 90 below).  In the forward four heads' plain
+// loads per turn do as well (61 us; the queue 64).
+//
+// B200, 16384 rows of 32 + 8 heads of 128, bf16: forward 61 us (5.5 TB/s, 84% of the copy rate),
+// backward 90 us (5.6 TB/s, 85%), the gains' sum included.
 #include <cuda_runtime.h>
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "mt_api.h"
 #include "vec_io.cuh"
@@ -27,6 +36,7 @@ namespace mt {
 namespace {
 
 constexpr int kWarps = 8;
+constexpr int kPerSm = 2;  // resident blocks: the kernels hold a head pair's values in about 128 registers
 constexpr int kMaxHalf = 128;
 
 // theta^(-2i/n) / (2 pi) as a product of the powers 2^k of the ratio theta^(-2/n): the host forms
@@ -62,8 +72,65 @@ __device__ __forceinline__ void row_turns(const double* freq, float* cs, float* 
   __syncwarp();
 }
 
+__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
+// What a thread reads in its coming turns: MATS matrices' two vectors of a head each, for `depth` turns.
+// Slots are [turn][vector part][thread]; fetch() is called once per turn and asks for the next one.
+template <class T, int MATS, int DEPTH>
+struct HeadQueue {
+  static constexpr int Q = sizeof(Raw8<T>) / 16, PARTS = 2 * MATS * Q;
+  uint4* slots;
+  const T* base[MATS];
+  long ld[MATS];
+  long row, rows, row_step;
+  int turn, turns, head, head_step, heads, half, hd, stage;
+  bool on;
+
+  __device__ __forceinline__ void fetch() {
+    if (row < rows) {
+      if (on && head < heads) {
+        uint4* c = slots + stage * PARTS * kWarps * 32;
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) {
+          const T* p = base[m] + row * ld[m] + (long)head * hd;
+#pragma unroll
+          for (int q = 0; q < Q; ++q) {
+            copy_async16(c + (m * 2 * Q + q) * kWarps * 32, (const char*)p + 16 * q);
+            copy_async16(c + (m * 2 * Q + Q + q) * kWarps * 32, (const char*)(p + half) + 16 * q);
+          }
+        }
+      }
+      head += head_step;
+      if (++turn == turns) {
+        turn = 0;
+        head -= turns * head_step;
+        row += row_step;
+      }
+    }
+    copy_async_commit();
+    stage = stage + 1 == DEPTH ? 0 : stage + 1;
+  }
+  // The oldest turn's vectors; its slots are the next fetch()'s.
+  __device__ __forceinline__ void read(int m, Raw8<T>& a, Raw8<T>& b) const {
+    const uint4* c = slots + (stage * PARTS + m * 2 * Q) * kWarps * 32;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      a.q[q] = c[q * kWarps * 32];
+      b.q[q] = c[(Q + q) * kWarps * 32];
+    }
+  }
+};
+
+// U heads per turn, their loads in flight together.
 template <class T, int G, int U>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, kPerSm)
     qk_norm_rope_fwd_kernel(const T* __restrict__ x, long ldx, const T* __restrict__ gq, const T* __restrict__ gk,
                             T* __restrict__ y, long ldy, int rows, int S, int H, int HK, int hd, float eps,
                             int warps_per_row, Turns turns) {
@@ -143,11 +210,12 @@ __global__ void __launch_bounds__(kWarps * 32)
 
 // The gain gradients of a block go to its row of `partial` [blocks][2][hd]; gain_sum_kernel adds the
 // rows in a fixed order, so that equal inputs give equal bits.
-template <class T, int G, int U>
-__global__ void __launch_bounds__(kWarps * 32)
+template <class T, int G, int DEPTH>
+__global__ void __launch_bounds__(kWarps * 32, kPerSm)
     qk_norm_rope_bwd_kernel(const T* dy, long lddy, const T* __restrict__ x, long ldx, const T* __restrict__ gq,
                             const T* __restrict__ gk, T* dx, long lddx, float* __restrict__ partial, int rows, int S,
                             int H, int HK, int hd, float eps, int warps_per_row, Turns turns) {
+  extern __shared__ uint4 ring[];
   __shared__ double freq[kMaxHalf];
   __shared__ float cs_all[kWarps][kMaxHalf], sn_all[kWarps][kMaxHalf];
   __shared__ float red[kWarps][2 * kMaxHalf];
@@ -160,89 +228,79 @@ __global__ void __launch_bounds__(kWarps * 32)
   const int slots = (32 / G) * warps_per_row;
   const int slot = (warp % warps_per_row) * (32 / G) + lane / G;
   const int rows_per_block = kWarps / warps_per_row;
+  const long row0 = (long)blockIdx.x * rows_per_block + warp / warps_per_row, row_step = (long)gridDim.x * rows_per_block;
   const float inv_n = 1.0f / (float)hd;
-  float acc[2][16];
-#pragma unroll
-  for (int j = 0; j < 16; ++j) acc[0][j] = acc[1][j] = 0.f;
-  for (long row = (long)blockIdx.x * rows_per_block + warp / warps_per_row; row < rows;
-       row += (long)gridDim.x * rows_per_block) {
-    row_turns(freq, cs_all[warp], sn_all[warp], half, (int)(row % S), lane);
-    float cs[8], sn[8];
-    if (on) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        cs[j] = cs_all[warp][d + j];
-        sn[j] = sn_all[warp][d + j];
-      }
-    }
-#pragma unroll
-    for (int part = 0; part < 2; ++part) {
-      const int n = part ? HK : H;
-      const T* gain = part ? gk : gq;
-      const long head0 = part ? (long)H * hd : 0;
-      const T* xr = x + row * ldx + head0 + d;
-      const T* gr = dy + row * lddy + head0 + d;
-      T* dxr = dx + row * lddx + head0 + d;
-      float ga[8], gb[8];
-      if (on) {
-        load8(gain + d, ga);
-        load8(gain + half + d, gb);
-      }
-      for (int h0 = 0; h0 < n; h0 += slots * U) {
-        Raw8<T> xa[U], xb[U], ya[U], yb[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int h = h0 + u * slots + slot;
-          if (on && h < n) {
-            xa[u] = ldraw8(xr + (long)h * hd);
-            xb[u] = ldraw8(xr + (long)h * hd + half);
-            ya[u] = ldraw8(gr + (long)h * hd);
-            yb[u] = ldraw8(gr + (long)h * hd + half);
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int h = h0 + u * slots + slot;
-          const bool mine = on && h < n;
-          float a[8], b[8], va[8], vb[8], ss = 0.f, dot = 0.f;
-          if (mine) {
-            float ea[8], eb[8];
-            unpack8(xa[u], a);
-            unpack8(xb[u], b);
-            unpack8(ya[u], ea);
-            unpack8(yb[u], eb);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              va[j] = ea[j] * cs[j] + eb[j] * sn[j];
-              vb[j] = eb[j] * cs[j] - ea[j] * sn[j];
-              ss += a[j] * a[j] + b[j] * b[j];
-              dot += va[j] * ga[j] * a[j] + vb[j] * gb[j] * b[j];
-            }
-          }
-          const float r = rsqrtf(group_sum<G>(ss) * inv_n + eps);
-          const float m = group_sum<G>(dot) * inv_n * r * r;  // mean(w x r) r
-          if (mine) {
-            float o1[8], o2[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              acc[part][j] += va[j] * a[j] * r;
-              acc[part][8 + j] += vb[j] * b[j] * r;
-              o1[j] = r * (va[j] * ga[j] - a[j] * m);
-              o2[j] = r * (vb[j] * gb[j] - b[j] * m);
-            }
-            store8(dxr + (long)h * hd, o1);
-            store8(dxr + (long)h * hd + half, o2);
-          }
-        }
-      }
-    }
-  }
-  // lanes that hold the same columns, then the block's warps, in a fixed order
-#pragma unroll
+#pragma unroll 1
   for (int part = 0; part < 2; ++part) {
+    const int n = part ? HK : H, its = (n + slots - 1) / slots;
+    const long first = (part ? (long)H * hd : 0) + d;
+    HeadQueue<T, 2, DEPTH> queue{ring + threadIdx.x, {x + first, dy + first}, {ldx, lddy}, row0, n ? rows : 0, row_step,
+                                 0, its, slot, slots, n, half, hd, 0, on};
+#pragma unroll
+    for (int k = 0; k < DEPTH; ++k) queue.fetch();
+    float ga[8], gb[8], acc[16];
+    if (on) {
+      load8((part ? gk : gq) + d, ga);
+      load8((part ? gk : gq) + half + d, gb);
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[j] = 0.f;
+    for (long row = row0; row < rows && n; row += row_step) {
+      row_turns(freq, cs_all[warp], sn_all[warp], half, (int)(row % S), lane);
+      float cs[8], sn[8];
+      if (on) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          cs[j] = cs_all[warp][d + j];
+          sn[j] = sn_all[warp][d + j];
+        }
+      }
+      T* dxr = dx + row * lddx + first;
+      for (int h = slot; h < its * slots; h += slots) {
+        copy_async_wait<DEPTH - 1>();
+        const bool mine = on && h < n;
+        float a[8], b[8], va[8], vb[8], ss = 0.f, dot = 0.f;
+        if (mine) {
+          Raw8<T> xa, xb, ya, yb;
+          float ea[8], eb[8];
+          queue.read(0, xa, xb);
+          queue.read(1, ya, yb);
+          unpack8(xa, a);
+          unpack8(xb, b);
+          unpack8(ya, ea);
+          unpack8(yb, eb);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            va[j] = ea[j] * cs[j] + eb[j] * sn[j];
+            vb[j] = eb[j] * cs[j] - ea[j] * sn[j];
+            ss += a[j] * a[j] + b[j] * b[j];
+            dot += va[j] * ga[j] * a[j] + vb[j] * gb[j] * b[j];
+          }
+        }
+        const float r = rsqrtf(group_sum<G>(ss) * inv_n + eps);
+        const float m = group_sum<G>(dot) * inv_n * r * r;  // mean(w x r) r
+        __syncwarp();
+        queue.fetch();
+        if (mine) {
+          float o1[8], o2[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float wa = va[j] * r, wb = vb[j] * r;
+            acc[j] += wa * a[j];
+            acc[8 + j] += wb * b[j];
+            o1[j] = wa * ga[j] - a[j] * (m * r);
+            o2[j] = wb * gb[j] - b[j] * (m * r);
+          }
+          store8(dxr + (long)h * hd, o1);
+          store8(dxr + (long)h * hd + half, o2);
+        }
+      }
+    }
+    copy_async_wait<0>();
+    // lanes that hold the same columns, then the block's warps, in a fixed order
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      float v = acc[part][j];
+      float v = acc[j];
 #pragma unroll
       for (int o = 16; o >= G; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
       if (lane < G && on) red[warp][(j < 8 ? 0 : half) + d + (j & 7)] = v;
@@ -258,23 +316,28 @@ __global__ void __launch_bounds__(kWarps * 32)
   }
 }
 
-constexpr int kSumCols = 32, kSumGroups = 32;
+// Sum of the blocks' partial gain gradients: 8 columns and 128 groups of rows per block, each thread's
+// few loads in flight together.
+constexpr int kSumCols = 8, kSumGroups = 128;
 
 __global__ void __launch_bounds__(kSumCols * kSumGroups)
     gain_sum_kernel(const float* __restrict__ partial, int blocks, int hd, float* __restrict__ dgq,
                     float* __restrict__ dgk) {
-  __shared__ float part[kSumGroups][kSumCols + 1];
-  const int c = threadIdx.x % kSumCols, g = threadIdx.x / kSumCols;
-  const int col = blockIdx.x * kSumCols + c;  // of 2 hd; hd is a multiple of 16
+  __shared__ float part[kSumCols * kSumGroups / 32][kSumCols];
+  const int c = threadIdx.x % kSumCols, g = threadIdx.x / kSumCols, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int col = blockIdx.x * kSumCols + c;  // of 2 hd, a multiple of kSumCols
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched ahead of the backward kernel's end
   float s = 0.f;
-  if (col < 2 * hd)
-    for (int b = g; b < blocks; b += kSumGroups) s += partial[(long)b * 2 * hd + col];
-  part[g][c] = s;
+#pragma unroll 4
+  for (int b = g; b < blocks; b += kSumGroups) s += partial[(long)b * 2 * hd + col];
+  s += __shfl_xor_sync(0xffffffffu, s, 8);
+  s += __shfl_xor_sync(0xffffffffu, s, 16);
+  if (lane < kSumCols) part[warp][c] = s;
   __syncthreads();
-  if (g == 0 && col < 2 * hd) {
+  if (threadIdx.x < kSumCols) {
     float t = 0.f;
 #pragma unroll
-    for (int k = 0; k < kSumGroups; ++k) t += part[k][c];
+    for (int w = 0; w < kSumCols * kSumGroups / 32; ++w) t += part[w][c];
     float* out = col < hd ? dgq + col : dgk + (col - hd);
     *out += t;
   }
@@ -288,10 +351,12 @@ Turns turns_of(int hd, double theta) {
   return t;
 }
 
-// Warps that share a row's heads: one, unless there are too few rows to fill the GPU with one each.
+// Warps that share a row's heads: one (a row's sines are computed by each), unless the rows fill less than
+// half of the GPU's warps with one each.  1000 rows of 32 + 8 heads of 128, forward / backward: 6.9 / 13.7 us
+// with this limit of 8 warps per SM, 7.5 / 15.8 with 16, 10.3 / 19.1 with 32.
 int warps_per_row_of(int rows, int heads, int slots, int sms) {
   int w = 1;
-  while (w < kWarps && (long)rows * w < 16L * sms && w * slots < heads) w *= 2;
+  while (w < kWarps && (long)rows * w < 8L * sms && w * slots < heads) w *= 2;
   return w;
 }
 
@@ -314,7 +379,21 @@ int with_lanes(int hd, F&& fn) {
 }
 
 int grid_of(int rows, int rows_per_block, int sms) {
-  return (int)std::min<long>(((long)rows + rows_per_block - 1) / rows_per_block, 4L * sms);
+  return (int)std::min<long>(((long)rows + rows_per_block - 1) / rows_per_block, (long)kPerSm * sms);
+}
+
+// Launch with `smem` bytes of dynamic shared memory, which is opted into once per kernel and device.
+template <class K, class... A>
+int launch(K kern, std::atomic<bool>* ready, int blocks, int smem, cudaStream_t s, A... args) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!ready[dev & 63].load()) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return (int)e;
+    ready[dev & 63].store(true);
+  }
+  kern<<<blocks, kWarps * 32, smem, s>>>(args...);
+  return (int)cudaGetLastError();
 }
 
 }  // namespace
@@ -330,16 +409,15 @@ int qk_norm_rope_fwd(const QkNormRopeArgs& a, cudaStream_t s) {
   if (a.hd % 16 || a.hd < 16 || a.hd > 2 * kMaxHalf || a.S < 1) return -1;
   if (a.rows == 0 || a.H + a.HK == 0) return 0;
   const int sms = sm_count();
-  const Turns turns = turns_of(a.hd, a.theta);
   return with_dtype(a.dtype, [&](auto v) {
     using T = decltype(v);
     return with_lanes(a.hd, [&](auto lanes) {
-      constexpr int G = decltype(lanes)::value;
+      constexpr int G = decltype(lanes)::value, U = sizeof(T) == 2 ? 4 : 2;  // 16 lines of 128 bytes per warp in flight
       const int w = warps_per_row_of(a.rows, a.H + a.HK, 32 / G, sms);
-      qk_norm_rope_fwd_kernel<T, G, sizeof(T) == 2 ? 2 : 1>
-          <<<grid_of(a.rows, kWarps / w, sms), kWarps * 32, 0, s>>>(
-              (const T*)a.x, a.ldx, (const T*)a.gq, (const T*)a.gk, (T*)a.out, a.ldo, a.rows, a.S, a.H, a.HK, a.hd,
-              a.eps, w, turns);
+      auto kern = w > 1 ? qk_norm_rope_fwd_kernel<T, G, 1> : qk_norm_rope_fwd_kernel<T, G, U>;
+      kern<<<grid_of(a.rows, kWarps / w, sms), kWarps * 32, 0, s>>>(
+          (const T*)a.x, a.ldx, (const T*)a.gq, (const T*)a.gk, (T*)a.out, a.ldo, a.rows, a.S, a.H, a.HK, a.hd, a.eps,
+          w, turns_of(a.hd, a.theta));
       return (int)cudaGetLastError();
     });
   });
@@ -350,19 +428,28 @@ int qk_norm_rope_bwd(const QkNormRopeArgs& a, const void* dy, long lddy, float* 
   if (a.hd % 16 || a.hd < 16 || a.hd > 2 * kMaxHalf || a.S < 1) return -1;
   if (a.rows == 0 || a.H + a.HK == 0) return 0;
   const int sms = sm_count();
-  const Turns turns = turns_of(a.hd, a.theta);
   return with_dtype(a.dtype, [&](auto v) {
     using T = decltype(v);
     return with_lanes(a.hd, [&](auto lanes) {
-      constexpr int G = decltype(lanes)::value;
+      constexpr int G = decltype(lanes)::value, DEPTH = sizeof(T) == 2 ? 3 : 2;
+      static std::atomic<bool> ready[64];
       const int w = warps_per_row_of(a.rows, a.H + a.HK, 32 / G, sms);
       const int blocks = grid_of(a.rows, kWarps / w, sms);
-      qk_norm_rope_bwd_kernel<T, G, 1><<<blocks, kWarps * 32, 0, s>>>(
-          (const T*)dy, lddy, (const T*)a.x, a.ldx, (const T*)a.gq, (const T*)a.gk, (T*)a.out, a.ldo, partial, a.rows,
-          a.S, a.H, a.HK, a.hd, a.eps, w, turns);
-      gain_sum_kernel<<<(2 * a.hd + kSumCols - 1) / kSumCols, kSumCols * kSumGroups, 0, s>>>(partial, blocks, a.hd,
-                                                                                             dgq, dgk);
-      return (int)cudaGetLastError();
+      const int rc = launch(qk_norm_rope_bwd_kernel<T, G, DEPTH>, ready, blocks,
+                            DEPTH * 4 * kWarps * 32 * (int)sizeof(Raw8<T>), s, (const T*)dy, lddy, (const T*)a.x, a.ldx,
+                            (const T*)a.gq, (const T*)a.gk, (T*)a.out, a.ldo, partial, a.rows, a.S, a.H, a.HK, a.hd,
+                            a.eps, w, turns_of(a.hd, a.theta));
+      if (rc) return rc;
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(2 * a.hd / kSumCols);
+      cfg.blockDim = dim3(kSumCols * kSumGroups);
+      cfg.stream = s;
+      cudaLaunchAttribute attr{};
+      attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr.val.programmaticStreamSerializationAllowed = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      return (int)cudaLaunchKernelEx(&cfg, gain_sum_kernel, (const float*)partial, blocks, a.hd, dgq, dgk);
     });
   });
 }
