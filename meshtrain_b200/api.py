@@ -174,7 +174,8 @@ class PipelineTrainer:
                  lr: float = 1e-3, weight_decay: float = 0.0, seed: int = 0, partition: str | list = "balanced",
                  max_inflight: int | None = None, device: str | None = None, init_on_device: bool = True,
                  offload=None, link_probe: bool = False, microbatch_size: int = 1, virtual_stages: int = 1,
-                 recompute=None, offload_options: dict | None = None, memory_gb: float | None = None):
+                 recompute=None, offload_options: dict | None = None, memory_gb: float | None = None,
+                 objective=None):
         """``partition``: "balanced" (FLOP-balanced DP), "topology_aware" (the planner, with memory
         budgets and NVLink links), "equal", or an explicit list of [start, end) layer ranges.
 
@@ -190,7 +191,10 @@ class PipelineTrainer:
         ``offload``: None (optimizer state on the GPU), a ``HostOffload``, or "auto": the
         startup memory estimate (``memory_gb`` per GPU, default this GPU's) decides, and a
         ``HostOffload(**offload_options)`` is made only if the stages do not fit with their
-        state resident (``parallel/placement.py``)."""
+        state resident (``parallel/placement.py``).
+
+        ``objective``: the loss instead of cross-entropy, a ``PreferenceObjective`` or ``PolicyObjective``
+        (``models/objectives.py``); its per-token tensors come with each ``step``."""
         self.rank, self.world, self.local_rank = init_distributed()
         self.spec = build_model_spec(model, seed=seed)
         n = self.spec.num_layers
@@ -292,7 +296,8 @@ class PipelineTrainer:
         self._engine_kw = dict(stage=self.stage, num_stages=self.world, device=self.device,
                                num_microbatches=num_microbatches, schedule=schedule, max_inflight=max_inflight,
                                optimizer=optimizer, lr=lr, weight_decay=weight_decay, links=links,
-                               init_on_device=init_on_device, microbatch_size=microbatch_size, recompute=rc)
+                               init_on_device=init_on_device, microbatch_size=microbatch_size, recompute=rc,
+                               objective=objective)
         self.engine = PipelineEngine(self.spec, layer_range=None if v > 1 else ranges[self.stage],
                                      chunk_ranges=self.chunk_ranges if v > 1 else None, offload=offload,
                                      **self._engine_kw)
@@ -382,15 +387,16 @@ class PipelineTrainer:
         return self.stage == self.world - 1
 
     def step(self, step: int, inputs: torch.Tensor | None, targets: torch.Tensor | None,
-             timed: bool | str = True) -> StepStats:
-        """One global step.  With several ranks a failure anywhere in the pipeline
+             timed: bool | str = True, extras: dict[str, torch.Tensor] | None = None) -> StepStats:
+        """One global step (``extras``: the per-token tensors of an ``objective``).  With several ranks a failure anywhere in the pipeline
         raises here (``PeerFailure`` on the ranks that did not fail) instead of
         leaving the survivors blocked in NCCL."""
         if self.watch is not None:
             self.watch.check()
         try:
             stats = self.engine.train_step(step, inputs if self.is_first else None,
-                                           targets if self.is_last else None, timed=timed)
+                                           targets if self.is_last else None, timed=timed,
+                                           extras=extras if self.is_last else None)
         except Exception as exc:
             if self.watch is not None:
                 from meshtrain_b200.parallel.watchdog import PeerFailure
@@ -403,6 +409,11 @@ class PipelineTrainer:
         if self.watch is not None:
             self.watch.beat(step)
         return stats
+
+    def logprobs(self, inputs: torch.Tensor | None, targets: torch.Tensor | None) -> torch.Tensor | None:
+        """Log probabilities [batch, S] of ``targets`` under the current weights (``PipelineEngine.logprobs``);
+        every rank calls it, the last one gets the result."""
+        return self.engine.logprobs(inputs if self.is_first else None, targets if self.is_last else None)
 
     def finish_timing(self, stats: list[StepStats]) -> list[StepStats]:
         """Device timing of steps run with ``timed="deferred"`` (waits for them)."""

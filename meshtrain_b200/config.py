@@ -4,7 +4,7 @@ The sections, key names and defaults are the reference's (config.py:16-215), so
 every reference YAML validates unchanged; that schema is an interface.  Keys
 added for the B200 build are optional: model types ``gpt`` / ``llama`` and
 their shape keys (``mlp_ratio``, ``n_kv_heads``, ``ffn_hidden``, ``rope_theta``,
-``init_std``, ``split_blocks``), ``data``, ``offload``,
+``init_std``, ``split_blocks``, ``qk_norm``, ``dropout``), ``data``, ``offload``,
 ``network.tensor_transport: nccl`` and ``kernels``, plus checkpointing keys
 under ``training``.
 
@@ -70,6 +70,13 @@ def _split_blocks_needs_blocks(m):
         return "split_blocks applies to gpt / tiny_transformer / llama models"
 
 
+def _block_options_need_blocks(m):
+    if m.qk_norm and m.type != "llama":
+        return "qk_norm applies to llama models"
+    if m.dropout is not None and (m.type == "mlp" or round(m.dropout * 65536) >= 65536):
+        return "dropout applies to gpt / tiny_transformer / llama models, and rounds (to 1/65536) below 1"
+
+
 class ModelConfig(_Section):
     type: Literal["mlp", "tiny_transformer", "gpt", "llama"]
     sizes: list[int] | None = None                 # mlp layer widths
@@ -85,8 +92,10 @@ class ModelConfig(_Section):
     rope_theta: float | None = Field(None, gt=0)
     init_std: float | None = Field(None, gt=0)
     split_blocks: bool = False                     # partition units of half a block (attention / MLP)
+    qk_norm: bool | None = None                    # llama: RMS norm of each query and key head before the rotation
+    dropout: float | None = Field(None, ge=0, lt=1)  # embedding output and residual branches
 
-    RULES = (_split_blocks_needs_blocks, _heads_divide_hidden, _mlp_sizes, _kv_heads_divide_heads)
+    RULES = (_split_blocks_needs_blocks, _block_options_need_blocks, _heads_divide_hidden, _mlp_sizes, _kv_heads_divide_heads)
 
     def spec_kwargs(self) -> dict:
         """Keyword arguments of the model registry for this model."""

@@ -43,6 +43,7 @@ def build_model_spec(cfg: dict, seed: int = 0) -> ModelSpec:
             mlp_ratio=cfg.get("mlp_ratio", 4),
             init_std=cfg.get("init_std"),
             data=data or ("arithmetic" if kind == "tiny_transformer" else "uniform"),
+            dropout=cfg.get("dropout", 0.0),
         )
     if kind == "llama":
         return LlamaSpec(
@@ -58,6 +59,8 @@ def build_model_spec(cfg: dict, seed: int = 0) -> ModelSpec:
             dtype=dtype,
             init_std=cfg.get("init_std", 0.02),
             data=data or "uniform",
+            qk_norm=cfg.get("qk_norm", False),
+            dropout=cfg.get("dropout", 0.0),
         )
     raise ValueError(f"unknown model type {kind!r}")
 

@@ -27,6 +27,10 @@ def layer_seed(seed: int, index: int) -> int:
     return (seed * 1_000_003 + index * 7919) % (2**31 - 1)
 
 
+RNG_KEY = "rng"  # saved[RNG_KEY]: (seed, offset) of a layer's random numbers in this pass
+RNG_SITES = 4    # offsets a layer may use from that one on
+
+
 class PipelineLayer(nn.Module):
     """A layer with an explicit forward/backward pair.
 
@@ -37,6 +41,20 @@ class PipelineLayer(nn.Module):
     """
 
     takes_integer_input = False
+    dropout = 0.0  # probability, of layers that have it
+
+    def dropping(self) -> bool:
+        return self.dropout > 0.0 and self.training
+
+    def _rng(self, saved: dict, site: int) -> tuple[int, int]:
+        """(seed, offset) of one use of random numbers in this pass, the same in its backward and in a
+        recomputed forward.  The engine puts them into ``saved`` from the run's seed, the step, the
+        microbatch and the layer; without it a pass draws them from torch's CPU generator."""
+        if RNG_KEY not in saved:
+            seed, base = torch.randint(0, 2**62, (2,)).tolist()
+            saved[RNG_KEY] = (seed, base * RNG_SITES % 2**62)
+        seed, offset = saved[RNG_KEY]
+        return seed, offset + site
 
     def fwd(self, x: torch.Tensor, saved: dict) -> torch.Tensor:  # pragma: no cover - abstract
         raise NotImplementedError

@@ -34,8 +34,9 @@ class Embedding(PipelineLayer):
     takes_integer_input = True
 
     def __init__(self, vocab_size: int, d_model: int, max_seq_len: int, init_std: float | None = None,
-                 learned_pos: bool = True):
+                 learned_pos: bool = True, dropout: float = 0.0):
         super().__init__()
+        self.dropout = dropout
         self.tok = nn.Embedding(vocab_size, d_model)
         self.pos = nn.Embedding(max_seq_len, d_model) if learned_pos else None
         self.seq_len = max_seq_len
@@ -47,17 +48,21 @@ class Embedding(PipelineLayer):
     def fwd(self, tokens, saved):
         B, S = tokens.shape
         out = ops.embedding(tokens, self.tok.weight, None if self.pos is None else self.pos.weight, S)
+        if self.dropping():
+            out = ops.dropout(out, self.dropout, *self._rng(saved, 2), out=out)
         saved["ids"] = tokens
         return out.view(B, S, -1)
 
     def bwd(self, dy, saved, grads):
         ids = saved["ids"]
         S = ids.shape[1]
+        if self.dropping():
+            dy = ops.dropout(dy, self.dropout, *self._rng(saved, 2))
         ops.embedding_bwd_(ids, dy, grads["tok.weight"], grads.get("pos.weight"), S)
         return None
 
     def forward(self, tokens):  # autograd path
-        if ops.backend() == "torch" or not tokens.is_cuda:
+        if (ops.backend() == "torch" or not tokens.is_cuda) and not self.dropping():
             positions = torch.arange(tokens.shape[1], device=tokens.device)
             out = self.tok(tokens)
             return out + self.pos(positions)[None] if self.pos is not None else out
@@ -66,8 +71,9 @@ class Embedding(PipelineLayer):
 
 class Block(PipelineLayer):
     def __init__(self, d_model: int, n_heads: int, mlp_ratio: int = 4, init_std: float | None = None,
-                 n_layers_for_scaling: int | None = None, eps: float = 1e-5):
+                 n_layers_for_scaling: int | None = None, eps: float = 1e-5, dropout: float = 0.0):
         super().__init__()
+        self.dropout = dropout
         if d_model % n_heads:
             raise ValueError("d_model must be divisible by n_heads")
         self.n_heads = n_heads
@@ -80,6 +86,18 @@ class Block(PipelineLayer):
         self.fc2 = nn.Linear(mlp_ratio * d_model, d_model)
         for lin in (self.qkv, self.proj, self.fc1, self.fc2):
             _init_linear(lin, init_std)
+
+    def _branch(self, y, lin, residual, saved, site):
+        """residual + dropout(lin(y)): one GEMM with the residual in its epilogue, or with dropout a GEMM and
+        one pass over its output."""
+        if not self.dropping():
+            return ops.linear(y, lin.weight, lin.bias, residual=residual)
+        h = ops.linear(y, lin.weight, lin.bias)
+        return ops.dropout(h, self.dropout, *self._rng(saved, site), residual=residual, out=h)
+
+    def _branch_grad(self, dy, saved, site):
+        """Gradient of that branch's linear output."""
+        return ops.dropout(dy, self.dropout, *self._rng(saved, site)) if self.dropping() else dy
 
     # The block is two residual halves; each half is also usable as a pipeline
     # layer of its own (models/split.py), so a stage boundary may fall between them.
@@ -96,7 +114,7 @@ class Block(PipelineLayer):
         k = qkv[:, d:2 * d].view(B, S, H, hd)
         v = qkv[:, 2 * d:].view(B, S, H, hd)
         o, lse = ops.attention(q, k, v, causal=True)
-        x1 = ops.linear(o.reshape(B * S, d), self.proj.weight, self.proj.bias, residual=x2)
+        x1 = self._branch(o.reshape(B * S, d), self.proj, x2, saved, 0)
         saved.update(shape=(B, S, d), x=x2, y1=y1, m1=m1, r1=r1, qkv=qkv, o=o, lse=lse)
         return x1.view(B, S, d)
 
@@ -105,15 +123,17 @@ class Block(PipelineLayer):
         x1 = x.reshape(B * S, d)
         y2, m2, r2 = ops.layernorm(x1, self.ln2.weight, self.ln2.bias, self.eps)
         g, h = ops.linear(y2, self.fc1.weight, self.fc1.bias, gelu=True)
-        out = ops.linear(g, self.fc2.weight, self.fc2.bias, residual=x1)
+        out = self._branch(g, self.fc2, x1, saved, 1)
         saved.update(shape=(B, S, d), x1=x1, y2=y2, m2=m2, r2=r2, h=h, g=g)
         return out.view(B, S, d)
 
     def mlp_bwd(self, dy, saved, grads):
         B, S, d = saved["shape"]
         dy2 = dy.reshape(B * S, d)
-        dh = ops.linear_dgrad(dy2, self.fc2.weight, gelu_pre=saved["h"])
-        ops.linear_wgrad_(dy2, saved["g"], grads["fc2.weight"], grads["fc2.bias"])
+        db = self._branch_grad(dy2, saved, 1)
+        dh = ops.linear_dgrad(db, self.fc2.weight, gelu_pre=saved["h"])
+        ops.linear_wgrad_(db, saved["g"], grads["fc2.weight"], grads["fc2.bias"])
+        del db
         dln2 = ops.linear_dgrad(dh, self.fc1.weight)
         ops.linear_wgrad_(dh, saved["y2"], grads["fc1.weight"], grads["fc1.bias"])
         del dh
@@ -127,8 +147,10 @@ class Block(PipelineLayer):
         hd = d // H
         T = B * S
         dx1 = dy.reshape(T, d)
-        do = ops.linear_dgrad(dx1, self.proj.weight)
-        ops.linear_wgrad_(dx1, saved["o"].reshape(T, d), grads["proj.weight"], grads["proj.bias"])
+        db = self._branch_grad(dx1, saved, 0)
+        do = ops.linear_dgrad(db, self.proj.weight)
+        ops.linear_wgrad_(db, saved["o"].reshape(T, d), grads["proj.weight"], grads["proj.bias"])
+        del db
         qkv = saved["qkv"]
         q = qkv[:, :d].view(B, S, H, hd)
         k = qkv[:, d:2 * d].view(B, S, H, hd)
@@ -162,7 +184,7 @@ class Block(PipelineLayer):
         return x + self.fc2(F.gelu(self.fc1(self.ln2(x))))
 
     def forward(self, x):  # autograd path
-        if ops.backend() == "torch" or not x.is_cuda:
+        if (ops.backend() == "torch" or not x.is_cuda) and not self.dropping():
             return self.mlp_torch(self.attn_torch(x))
         return super().forward(x)
 
@@ -220,30 +242,122 @@ class LMHead(PipelineLayer):
         accumulated with the mean-CE gradient times ``grad_scale``; the input
         gradient is kept in ``saved["dx"]`` for ``bwd_from_loss``.
         """
+        T = x.shape[0] * x.shape[1]
+        tg = targets.reshape(T)
+
+        def cross_entropy(lg, c0, c1):
+            ops.cross_entropy_chunk_(lg, self.vocab, tg[c0:c1], loss_sum, 1.0 / T, grad_scale / T)
+
+        self._chunked_loss(x, saved, grads, cross_entropy, chunk_tokens)
+
+    def _chunk_tokens(self, T: int) -> int:
+        """Tokens whose logits fit one GiB of bf16, at least 128."""
+        return max(128, min(T, (1 << 30) // ((self.vocab + 7) // 8 * 8 * 2)))
+
+    def _logits_buffer(self, y, chunk_tokens):
+        return torch.empty(min(chunk_tokens, y.shape[0]), (self.vocab + 7) // 8 * 8, device=y.device, dtype=y.dtype)
+
+    def _logits(self, yc, lg):
+        """Logits of normalised rows ``yc`` into ``lg`` (rows padded to a multiple of 8 columns)."""
+        if ops._custom(yc, self.out.weight):
+            ops.extension().gemm(yc, False, self.out.weight, False, lg, ops.EPI_BF16, self.out.bias, None, None, 0.0)
+        else:
+            lg[:, :self.vocab] = ops.linear(yc, self.out.weight, self.out.bias)
+
+    def _chunked_loss(self, x, saved, grads, to_gradient, chunk_tokens=None, normed=None, logits=None) -> None:
+        """Logits, their gradient and the layer's backward, a chunk of tokens at a time.
+
+        ``to_gradient(lg, c0, c1)`` replaces the logits of rows [c0, c1) by their gradient.  ``normed``: the
+        norm's result where a pass before needed it; ``logits``: all rows' logits where it kept them."""
         B, S, d = x.shape
         T = B * S
-        V = self.vocab
         x2 = x.reshape(T, d)
-        tg = targets.reshape(T)
-        y, m, r = self._norm(x2)
-        vpad = (V + 7) // 8 * 8
-        if chunk_tokens is None:
-            chunk_tokens = max(128, min(T, (1 << 30) // (vpad * 2)))
+        y, m, r = self._norm(x2) if normed is None else normed
+        chunk_tokens = chunk_tokens or self._chunk_tokens(T)
         dy = torch.empty_like(x2)
-        logits = torch.empty(min(chunk_tokens, T), vpad, device=x.device, dtype=x.dtype)
+        buf = self._logits_buffer(y, chunk_tokens) if logits is None else logits
         for c0 in range(0, T, chunk_tokens):
             c1 = min(T, c0 + chunk_tokens)
-            lg = logits[: c1 - c0]
+            lg = buf[: c1 - c0]
             yc = y[c0:c1]
-            if ops._custom(yc, self.out.weight):
-                ops.extension().gemm(yc, False, self.out.weight, False, lg, ops.EPI_BF16, self.out.bias, None, None, 0.0)
-            else:
-                lg[:, :V] = ops.linear(yc, self.out.weight, self.out.bias)
-            ops.cross_entropy_chunk_(lg, V, tg[c0:c1], loss_sum, 1.0 / T, grad_scale / T)
-            dl = lg[:, :V]
+            if logits is None:
+                self._logits(yc, lg)
+            to_gradient(lg, c0, c1)
+            dl = lg[:, :self.vocab]
             ops.linear_dgrad(dl, self.out.weight, out=dy[c0:c1])  # straight into this chunk's rows
             ops.linear_wgrad_(dl, yc, grads["out.weight"], grads.get("out.bias"))
         saved["dx"] = self._norm_bwd(dy, x2, m, r, grads).view(B, S, d)
+
+    def logprobs(self, x, targets, chunk_tokens: int | None = None) -> torch.Tensor:
+        """Log probabilities [B, S] (fp32) of the targets; 0 where a target is outside the vocabulary."""
+        B, S, d = x.shape
+        T = B * S
+        tg = targets.reshape(T)
+        y = self._norm(x.reshape(T, d))[0]
+        chunk_tokens = chunk_tokens or self._chunk_tokens(T)
+        buf = self._logits_buffer(y, chunk_tokens)
+        out = torch.empty(T, device=x.device, dtype=torch.float32)
+        for c0 in range(0, T, chunk_tokens):
+            c1 = min(T, c0 + chunk_tokens)
+            lg = buf[: c1 - c0]
+            self._logits(y[c0:c1], lg)
+            out[c0:c1] = ops.token_logprobs(lg, self.vocab, tg[c0:c1])[0]
+        return out.view(B, S)
+
+    def fwd_policy_loss(self, x, targets, saved, grads, loss_sum: torch.Tensor, grad_scale: float, *, old_logps,
+                        advantages, mask, ref_logps=None, clip_low: float = 0.2, clip_high: float = 0.2,
+                        kl_coef: float = 0.0, chunk_tokens: int | None = None) -> None:
+        """``fwd_loss`` with the clipped policy loss (``ops.policy_loss_chunk``), averaged over the tokens
+        that ``mask`` marks; all per-token tensors are [B, S]."""
+        T = x.shape[0] * x.shape[1]
+        flat = lambda t: None if t is None else t.reshape(T)  # noqa: E731
+        tg, old, ref, adv = flat(targets), flat(old_logps), flat(ref_logps), flat(advantages)
+        w = flat(mask).to(torch.float32)
+        w = w / w.sum().clamp(min=1.0)
+
+        def policy(lg, c0, c1):
+            part = slice(c0, c1)
+            losses, _, _ = ops.policy_loss_chunk(lg, self.vocab, tg[part], old[part], adv[part], w[part],
+                                                 ref_logps=None if ref is None else ref[part], clip_low=clip_low,
+                                                 clip_high=clip_high, kl_coef=kl_coef, grad_scale=grad_scale, out=lg)
+            loss_sum.add_(losses.sum())
+
+        self._chunked_loss(x, saved, grads, policy, chunk_tokens)
+
+    def fwd_preference_loss(self, x, targets, saved, grads, loss_sum: torch.Tensor, grad_scale: float, *, ref_logps,
+                            mask, beta: float = 0.1, form: str = "sigmoid", label_smoothing: float = 0.0,
+                            chunk_tokens: int | None = None) -> None:
+        """``fwd_loss`` with the preference loss (``ops.preference_loss``), averaged over the pairs: rows 2i and
+        2i + 1 of the microbatch are pair i's preferred and rejected answer.
+
+        A row's gradient needs its whole answer's log probability, so the logits are passed over twice: kept
+        between the passes if one chunk holds them all, formed again by a second GEMM otherwise."""
+        B, S, d = x.shape
+        if B % 2:
+            raise ValueError("the preference loss needs an even microbatch size: pairs are adjacent rows")
+        T = B * S
+        tg = targets.reshape(T)
+        normed = self._norm(x.reshape(T, d))
+        y = normed[0]
+        chunk_tokens = chunk_tokens or self._chunk_tokens(T)
+        buf = self._logits_buffer(y, chunk_tokens)
+        acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+        logps = torch.empty(T, device=x.device, dtype=acc)
+        stats = torch.empty(T, 2, device=x.device, dtype=acc)
+        for c0 in range(0, T, chunk_tokens):
+            c1 = min(T, c0 + chunk_tokens)
+            lg = buf[: c1 - c0]
+            self._logits(y[c0:c1], lg)
+            logps[c0:c1], stats[c0:c1] = ops.token_logprobs(lg, self.vocab, tg[c0:c1])
+        losses, _, dlogps = ops.preference_loss(logps.view(B, S), ref_logps, mask, beta, form=form,
+                                                label_smoothing=label_smoothing, grad_scale=grad_scale / (B // 2))
+        loss_sum.add_(losses.mean())
+        dlogps = dlogps.view(T)
+
+        def backward(lg, c0, c1):
+            ops.token_logprobs_bwd(lg, self.vocab, tg[c0:c1], stats[c0:c1], dlogps[c0:c1], out=lg)
+
+        self._chunked_loss(x, saved, grads, backward, chunk_tokens, normed, buf if T <= chunk_tokens else None)
 
     def forward(self, x):  # autograd path
         if ops.backend() == "torch" or not x.is_cuda:
@@ -272,8 +386,9 @@ class GPTSpec(ModelSpec):
 
     def __init__(self, layers: int = 6, hidden_size: int = 256, heads: int = 4, vocab_size: int = 256,
                  seq_len: int = 64, seed: int = 0, dtype: torch.dtype = torch.float32, mlp_ratio: int = 4,
-                 init_std: float | None = None, data: str = "arithmetic"):
+                 init_std: float | None = None, data: str = "arithmetic", dropout: float = 0.0):
         super().__init__(seed, dtype)
+        self.dropout = dropout  # of the embedding's output and of every residual branch
         self.n_blocks = layers
         self.d_model = hidden_size
         self.n_heads = heads
@@ -296,10 +411,10 @@ class GPTSpec(ModelSpec):
 
     def _make_layer(self, index: int) -> nn.Module:
         if index == 0:
-            return Embedding(self.vocab_size, self.d_model, self.seq_len, self.init_std)
+            return Embedding(self.vocab_size, self.d_model, self.seq_len, self.init_std, dropout=self.dropout)
         if index == self.num_layers - 1:
             return LMHead(self.d_model, self.vocab_size, self.init_std)
-        return Block(self.d_model, self.n_heads, self.mlp_ratio, self.init_std)
+        return Block(self.d_model, self.n_heads, self.mlp_ratio, self.init_std, dropout=self.dropout)
 
     def loss_fn(self, output, target):
         return F.cross_entropy(output.reshape(-1, output.shape[-1]).float(), target.reshape(-1))

@@ -37,6 +37,14 @@ class BlockHalf(PipelineLayer):
             self.add_module(name, getattr(block, name))
         self.__dict__["_block"] = block  # the arithmetic lives on the block; not a registered submodule
 
+    @property
+    def dropout(self) -> float:
+        return self._block.dropout
+
+    def train(self, mode: bool = True):
+        self._block.training = mode  # the arithmetic asks the block
+        return super().train(mode)
+
     def fwd(self, x, saved):
         b = self._block
         return b.attn_fwd(x, saved) if self.which == 0 else b.mlp_fwd(x, saved)
@@ -47,7 +55,8 @@ class BlockHalf(PipelineLayer):
 
     def forward(self, x):
         b = self._block
-        torch_path = getattr(b, "attn_torch", None) is not None and (ops.backend() == "torch" or not x.is_cuda)
+        torch_path = (getattr(b, "attn_torch", None) is not None and (ops.backend() == "torch" or not x.is_cuda)
+                      and not b.dropping())
         if torch_path:
             return b.attn_torch(x) if self.which == 0 else b.mlp_torch(x)
         return super().forward(x)

@@ -508,7 +508,8 @@ def qk_norm_rope(qkv, q_gain, k_gain, seq_len: int, heads: int, kv_heads: int, h
     ``qkv`` [T, >= (heads + kv_heads) * head_dim] holds the query heads, then the key heads (columns
     behind them are not read); row t has position t % seq_len.  Each head is scaled by
     ``(mean(x^2) + eps)^-1/2`` times ``q_gain`` / ``k_gain`` [head_dim] and rotated as ``rope_`` does.
-    Returns [T, (heads + kv_heads) * head_dim]; ``qkv`` itself is what the backward needs.
+    Returns [T, (heads + kv_heads) * head_dim], in ``out`` when given, which must not overlap ``qkv``:
+    that is what the backward needs.
     """
     if _custom_float(qkv):
         return _EXT.qk_norm_rope_fwd(qkv, q_gain, k_gain, seq_len, heads, kv_heads, head_dim, theta, eps, out)

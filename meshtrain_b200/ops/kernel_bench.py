@@ -223,6 +223,61 @@ def cases():
 
     out["cross_entropy_fwd_bwd"] = ce(2048, 50257, 50264)
 
+    def qk_norm_rope(T, S, H, HK, hd, bwd):
+        nbytes = (3 if bwd else 2) * T * (H + HK) * hd * 2
+
+        def make():
+            qkv, dqkv = _bf(T, (H + 2 * HK) * hd), _bf(T, (H + 2 * HK) * hd)
+            gq, gk, dg = _bf(hd), _bf(hd), torch.zeros(2, hd, device="cuda")
+            shape = (S, H, HK, hd, 500000.0)
+            if bwd:
+                return lambda: ops.qk_norm_rope_bwd(dqkv, qkv, gq, gk, *shape, dg[0], dg[1], out=dqkv)
+            return lambda: ops.qk_norm_rope(qkv, gq, gk, *shape)
+
+        def setup():
+            return rotating(make, nbytes), 0.0, nbytes
+        return setup
+
+    out["qk_norm_rope_fwd"] = qk_norm_rope(4096, 4096, 32, 8, 128, False)
+    out["qk_norm_rope_bwd"] = qk_norm_rope(4096, 4096, 32, 8, 128, True)
+
+    def dropout(T, d, residual):
+        nbytes = (3 if residual else 2) * T * d * 2
+
+        def make():
+            x, res = _bf(T, d), _bf(T, d) if residual else None
+            return lambda: ops.dropout(x, 0.1, 1, 2, residual=res, out=x)
+
+        def setup():
+            return rotating(make, nbytes), 0.0, nbytes
+        return setup
+
+    out["dropout_residual"] = dropout(T, 1280, True)
+    out["dropout_grad_d4096"] = dropout(4096, 4096, False)
+
+    def token_loss(T, V, kind):
+        vpad = (V + 7) // 8 * 8
+        nbytes = (1 if kind == "logprobs" else 2) * T * vpad * 2
+
+        def make():
+            logits, y = _bf(T, vpad), torch.randint(0, V, (T,), device="cuda")
+            lp, stats = ops.token_logprobs(logits, V, y)
+            one, out_ = torch.ones_like(lp), torch.empty_like(logits)
+            if kind == "logprobs":
+                return lambda: ops.token_logprobs(logits, V, y)
+            if kind == "bwd":
+                return lambda: ops.token_logprobs_bwd(logits, V, y, stats, one, out=out_)
+            return lambda: ops.policy_loss_chunk(logits, V, y, lp, one, one, ref_logps=lp, kl_coef=0.1, out=out_)
+
+        def setup():
+            return rotating(make, nbytes), 0.0, nbytes
+        return setup
+
+    out["token_logprobs"] = token_loss(4096, 50257, "logprobs")
+    out["token_logprobs_bwd"] = token_loss(4096, 50257, "bwd")
+    out["policy_loss"] = token_loss(4096, 50257, "policy")
+    out["policy_loss_v128256"] = token_loss(4096, 128256, "policy")
+
     def adam(n):
         def setup():
             p, g = torch.randn(n, device="cuda"), torch.randn(n, device="cuda")

@@ -31,7 +31,7 @@ import torch
 from torch import nn
 
 from meshtrain_b200 import ops
-from meshtrain_b200.models.base import ModelSpec
+from meshtrain_b200.models.base import RNG_KEY, RNG_SITES, ModelSpec
 from meshtrain_b200.parallel.schedule import ActionKind, ChunkAction, ChunkLedger, StepLedger, stage_schedule
 
 ALIGN = 64  # elements; keeps every parameter view 128-byte aligned for TMA
@@ -201,11 +201,12 @@ class PipelineEngine:
                  links=None, init_on_device: bool = False,
                  record_spans: bool = True, offload=None, microbatch_size: int | None = None,
                  deferred_wgrad: bool = True, chunk_ranges: list[tuple[int, int]] | None = None,
-                 recompute: set[int] | None = None):
+                 recompute: set[int] | None = None, objective=None):
         """``chunk_ranges``: the rank's model chunks for an interleaved 1F1B program (chunk c
         of this rank is virtual stage c * num_stages + stage); ``layer_range`` otherwise.
         ``recompute``: global units whose activations are recomputed in backward instead of
-        kept (``parallel/recompute.py``)."""
+        kept (``parallel/recompute.py``).  ``objective``: the loss of the last layer instead of
+        cross-entropy (``models/objectives.py``); its per-token inputs come with each step."""
         self.spec = spec
         self.deferred_wgrad = deferred_wgrad  # weight-gradient GEMMs on a side stream (CUDA)
         self.microbatch_size = microbatch_size  # middle stages see neither inputs nor targets
@@ -248,6 +249,11 @@ class PipelineEngine:
         self._spare_pools: list[_Events] = []  # event pools of finished deferred-timing steps
         self.record_spans = record_spans
         self._has_fused_loss = hasattr(self.layers[-1], "fwd_loss")
+        self.objective = objective
+        if objective is not None and self.is_last and not self._has_fused_loss:
+            raise ValueError("an objective needs a model whose last layer is an LM head")
+        self._pass = (0, 0)  # step and microbatch of the forward under way
+        self._rng_layers = sum(1 for i in range(spec.num_layers) if i == 0 or spec.global_layer(i) != spec.global_layer(i - 1))
         self.failure_check = None  # () -> reason or None: set by a trainer that watches its peers
         # NVTX ranges per action and for the optimizer (MESHTRAIN_NVTX=1), for Nsight timelines
         self.nvtx = os.environ.get("MESHTRAIN_NVTX") == "1"
@@ -275,11 +281,21 @@ class PipelineEngine:
     def _recv_buf(self, mb_size: int) -> torch.Tensor:
         return torch.empty(self.boundary_shape(mb_size), dtype=self.compute_dtype, device=self.device)
 
+    def _random_numbers(self, li: int, sv: dict) -> None:
+        """Seed and offset of a layer's dropout in this pass: a function of the run's seed, the step, the
+        microbatch and the layer of the model, so the same on any stage split and in a recomputed forward."""
+        if getattr(self.layers[li], "dropout", 0.0):
+            layer = self.spec.global_layer(self.layer_ids[li])
+            step, mb = self._pass
+            offset = ((step * self.M + mb) * self._rng_layers + layer) * RNG_SITES
+            sv[RNG_KEY] = (self.spec.seed % 2**64, offset % 2**62)
+
     def _forward_layers(self, x, saved_list, lo, hi):
         for li, sv in zip(range(lo, hi), saved_list):
+            self._random_numbers(li, sv)
             if li in self.recompute_local:
                 # keep only the input; the backward runs this forward again (_rematerialise)
-                x_in, x = x, self.layers[li].fwd(x, {})
+                x_in, x = x, self.layers[li].fwd(x, dict(sv))
                 sv[_RECOMPUTE_INPUT] = x_in
             else:
                 x = self.layers[li].fwd(x, sv)
@@ -308,9 +324,12 @@ class PipelineEngine:
             return vs if sender else vs - 1
         return vs - 1 if sender else vs
 
-    def _last_forward_loss(self, h, y, saved_list):
+    def _last_forward_loss(self, h, y, saved_list, extras=None):
         head = self.layers[-1]
         grads = self.flat.grads[-1]
+        if self.objective is not None:
+            self.objective.apply(head, h, y, extras, saved_list[-1], grads, self.loss_sum, 1.0 / self.M)
+            return
         if self._has_fused_loss:
             head.fwd_loss(h, y, saved_list[-1], grads, self.loss_sum, 1.0 / self.M)
             return
@@ -341,7 +360,7 @@ class PipelineEngine:
 
     # ------------------------------------------------------------------ step
     def train_step(self, step: int, inputs: torch.Tensor | None = None, targets: torch.Tensor | None = None,
-                   timed: bool | str = True) -> StepStats:
+                   timed: bool | str = True, extras: dict[str, torch.Tensor] | None = None) -> StepStats:
         """One global step: M microbatches through the schedule, then the optimizer.
 
         ``inputs`` (first stage) / ``targets`` (last stage) are the global
@@ -349,6 +368,7 @@ class PipelineEngine:
         ``timed``: True waits for the step and fills its device timing;
         "deferred" records the same events without waiting (the host runs on
         into the next step) and ``finish_timing(stats)`` fills them later.
+        ``extras`` (last stage, with an ``objective``): its per-token tensors, batched as the targets.
         """
         M = self.M
         dev = self.device
@@ -360,6 +380,11 @@ class PipelineEngine:
             if targets is None:
                 raise ValueError("the last stage needs targets")
             ys = targets.to(dev, non_blocking=True).chunk(M)
+            es = [None] * M
+            if self.objective is None and extras:
+                raise ValueError("extras are an objective's: this engine has none")
+            if self.objective is not None:
+                es = self.objective.split(extras, targets, M, dev)
         if inputs is not None or targets is not None:
             batch = (inputs if inputs is not None else targets).shape[0]
         elif self.microbatch_size is not None:
@@ -449,9 +474,10 @@ class PipelineEngine:
                 if a.kind is ActionKind.FORWARD:
                     x = xs[mb] if self.first_virtual(c) else buf
                     sv = [dict() for _ in range(hi - lo)]
+                    self._pass = (step, mb)
                     h = self._forward_layers(x, sv, lo, hi_fwd)
                     if last:
-                        self._last_forward_loss(h, ys[mb], sv)
+                        self._last_forward_loss(h, ys[mb], sv, es[mb])
                     else:
                         key = msg_key("F", mb, c, True)
                         sends.append((key, links.send_activation(h) if self.stage < S - 1
@@ -506,6 +532,45 @@ class PipelineEngine:
             self.wait_event(e_opt1)
             self._fill_timing(stats, t0, marks, e_opt0, e_opt1, side.spans if side else [], sends)
         return stats
+
+    @torch.no_grad()
+    def logprobs(self, inputs: torch.Tensor | None = None, targets: torch.Tensor | None = None) -> torch.Tensor | None:
+        """Log probabilities [batch, S] of ``targets`` under the current weights, without dropout, on the last
+        stage (None elsewhere): what a preference or policy objective takes as its reference or old log
+        probabilities.  Every stage calls it; microbatch by microbatch, forward only."""
+        if self.chunks > 1:
+            raise ValueError("logprobs needs one model chunk per rank")
+        if not hasattr(self.layers[-1], "logprobs") and self.is_last:
+            raise ValueError("logprobs needs a model whose last layer is an LM head")
+        M, dev = self.M, self.device
+        batch = inputs if self.is_first else targets if self.is_last else None
+        if (self.is_first and inputs is None) or (self.is_last and targets is None):
+            raise ValueError("the first stage needs inputs, the last needs targets")
+        rows = self.microbatch_size * M if batch is None else batch.shape[0]
+        if rows % M:
+            raise ValueError("batch size must be divisible by the number of microbatches")
+        out = []
+        modes = [layer.training for layer in self.layers]
+        for layer in self.layers:
+            layer.train(False)
+        try:
+            for mb in range(M):
+                part = slice(mb * (rows // M), (mb + 1) * (rows // M))
+                if self.is_first:
+                    x = inputs[part].to(dev, non_blocking=True)
+                else:
+                    x = self._recv_buf(rows // M)
+                    self.links.recv_activation(x).wait()
+                for layer in self.layers[:-1] if self.is_last else self.layers:
+                    x = layer.fwd(x, {})
+                if self.is_last:
+                    out.append(self.layers[-1].logprobs(x, targets[part].to(dev, non_blocking=True)))
+                else:
+                    self.links.send_activation(x).wait()
+        finally:
+            for layer, mode in zip(self.layers, modes):
+                layer.train(mode)
+        return torch.cat(out) if self.is_last else None
 
     def finish_timing(self, stats: StepStats) -> StepStats:
         """Fills the device timing of a step run with ``timed="deferred"`` (waits for it)."""

@@ -92,6 +92,8 @@ def analytic_profile(spec, microbatch_size: int) -> list[LayerProfile]:
             else:
                 hd = d // spec.n_heads
                 qkv = (spec.n_heads + 2 * spec.n_kv_heads) * hd
+                if getattr(spec, "qk_norm", False):  # normalised and rotated heads beside the projection's
+                    qkv += (spec.n_heads + spec.n_kv_heads) * hd
                 attn = T * eb * (d + d + qkv + d) + T * 4 * (1 + spec.n_heads)
                 mlp = T * eb * (d + d + 3 * spec.ffn_hidden) + T * 4
             if getattr(spec, "split_blocks", False):
