@@ -19,9 +19,10 @@
 //     which a cluster splits.
 //   stream_logprobs_kernel: many wide rows, statistics only.  4096 x 50257 bf16: 72 us, 5.7 TB/s (87% of
 //     the copy rate); 4096 x 128256: 166 us, 6.3 TB/s.
-//   stream_policy_kernel: many wide rows, statistics and gradient from one reading.  4096 x 128256 bf16:
-//     455 us, 4.6 TB/s (71%; half of such a row is read again, from L2); 8192 x 50257: 327 us, 5.0 TB/s.
-//     It computes two exponentials per logit, on a unit that does 16 per SM and clock: 55% of its time.
+//   stream_policy_kernel: many wide rows, statistics and gradient from one reading.  8192 x 50257 bf16:
+//     304 us, 5.4 TB/s (83%); 4096 x 128256: 413 us, 5.1 TB/s (78%; a tenth of such a row is read again,
+//     from L2).  It computes two exponentials per logit, on a unit that does 16 per SM and clock, for
+//     60% of its time, and waits twice per row for the row's statistic.
 #include <cuda_runtime.h>
 #include <math.h>
 
@@ -554,7 +555,7 @@ __global__ void __launch_bounds__(NT + 32, 1024 / NT) stream_logprobs_kernel(Row
 // kLag rounds ago join the next row's statistic.  Each thread only ever touches its own slots, so the
 // loop has no barrier; reads and writes of DRAM run side by side.  Columns that do not fit are read by
 // a pass of their own before the row's statistic is complete, and right after it again, from L2.
-constexpr int kLag = 3;
+constexpr int kLag = 2;
 
 // The same with 32-bit shared addresses, which the compiler offsets by literals.
 __device__ __forceinline__ uint4 shared_load16(uint32_t at) {
@@ -574,8 +575,12 @@ __device__ __forceinline__ void copy_async_small(void* dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
 }
 
+// Blocks of the policy kernel per SM: 768 threads (640 in one), so that each has 85 registers or more.  With 1024
+// threads of 64, V = 50257 (8192 rows) took 327 us instead of 305.
+constexpr int policy_blocks(int NT) { return NT > 400 ? 1 : NT > 256 ? 2 : NT > 128 ? 3 : 6; }
+
 template <class T, int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) stream_policy_kernel(RowArgs a, int cached) {
+__global__ void __launch_bounds__(NT, policy_blocks(NT)) stream_policy_kernel(RowArgs a, int cached) {
   extern __shared__ uint4 cache[];  // [part of a vector][cached]
   constexpr int W = NT / 32, NV = sizeof(T) == 2 ? 2 : 1, ROUND = NV * NT, Q = sizeof(Raw8<T>) / 16;
   __shared__ float2 pairs[2][W];
@@ -686,15 +691,16 @@ __global__ void __launch_bounds__(NT, 1024 / NT) stream_policy_kernel(RowArgs a,
         }
         return r;
       };
-      for (int v0 = cached; v0 < full; v0 += ROUND) {
+      for (int v0 = cached; v0 < full; v0 += 2 * ROUND) {
         const long at = (long)(v0 + tid) * 8;
-        Raw8<T> raw[NV];
+        const int rest = full - v0 - tid;
+        Raw8<T> raw[2 * NV];
 #pragma unroll
-        for (int u = 0; u < NV; ++u)
-          if (v0 + u * NT + tid < full) raw[u] = ldraw8(x + at + u * NT * 8);
+        for (int u = 0; u < 2 * NV; ++u)
+          if (u * NT < rest) raw[u] = ldraw8(x + at + u * NT * 8);
 #pragma unroll
-        for (int u = 0; u < NV; ++u)
-          if (v0 + u * NT + tid < full) straw8(out + at + u * NT * 8, turned(raw[u]));
+        for (int u = 0; u < 2 * NV; ++u)
+          if (u * NT < rest) straw8(out + at + u * NT * 8, turned(raw[u]));
       }
       uint32_t at = mine;
       T* o = out + tid * 8;
@@ -942,11 +948,11 @@ int sm_count(int* sms) {
 }
 
 // A block's share of the SM's shared memory when 1024 / NT blocks run on it.
-constexpr int cache_bytes(int NT) { return (224 << 10) / (1024 / NT) - 1024 - 256; }
+constexpr int cache_bytes(int NT) { return ((224 << 10) / policy_blocks(NT) - 1024 - 256) / 64 * 64; }
 
 template <class T, bool POLICY, int NT>
 int launch_stream(const RowArgs& a, int sms, cudaStream_t s) {
-  const int blocks = (int)std::min<long>(a.rows, (long)sms * (1024 / NT));
+  const int blocks = (int)std::min<long>(a.rows, (long)sms * (POLICY ? policy_blocks(NT) : 1024 / NT));
   if constexpr (POLICY) {
     constexpr int most = cache_bytes(NT) / (int)sizeof(Raw8<T>);
     auto kern = stream_policy_kernel<T, NT>;
@@ -985,14 +991,19 @@ int dispatch_rows(const RowArgs& a, cudaStream_t s) {
       // 128 / 256 / 512 threads: V = 50257 (8192 rows) 184 / 141 / 159 us, 128256 (4096 rows) 224 / 171 / 171
       return launch_stream<T, POLICY, 256>(a, sms, s);
     } else {
-      // small blocks for narrow rows: more rows are under way at once, which covers the barriers, until
-      // much of a row has to be read twice.  B200, us with 128 / 256 / 512 threads:
-      //   V = 16384 (16384 rows) 206 / 217 / 302    32000 (8192 rows) 230 / 198 / 239
-      //   V = 50257 (8192 rows)  434 / 339 / 327   128256 (4096 rows) 568 / 525 / 454
+      // Small blocks for narrow rows: more rows are under way at once, which covers the barriers, until
+      // much of a row has to be read twice.  B200, bf16, us with 128 / 256 / 384 / 640 threads:
+      //   V = 16384 (16384 rows) 183 / 228 / 286 / 455
+      //   V = 32000 (8192 rows)  211 / 194 / 212 / 310
+      //   V = 50257 (8192 rows)  397 / 310 / 304 / 406
+      //   V = 100000 (4096 rows) 468 / 398 / 342 / 329
+      //   V = 128256 (4096 rows) 612 / 527 / 448 / 414
+      // fp32 rows take 384 threads at most: 393 us at V = 50257 (4096 rows), 443 with 640.
       const long bytes = (long)V * sizeof(T);
       if (bytes <= cache_bytes(128) * 5L / 4) return launch_stream<T, POLICY, 128>(a, sms, s);
       if (bytes <= cache_bytes(256) * 5L / 4) return launch_stream<T, POLICY, 256>(a, sms, s);
-      return launch_stream<T, POLICY, 512>(a, sms, s);
+      if (sizeof(T) == 4 || bytes <= cache_bytes(384) * 3L / 2) return launch_stream<T, POLICY, 384>(a, sms, s);
+      return launch_stream<T, POLICY, 640>(a, sms, s);
     }
   }
   while (need < 8 && (long)a.rows * need <= sms && V / (2 * need) >= 2048) need *= 2;
