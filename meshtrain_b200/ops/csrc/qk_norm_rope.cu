@@ -14,14 +14,13 @@
 // is spread over G lanes, each holding 8 adjacent values of either half, so that the rotation's pairs
 // meet in one thread, every access is a 16-byte vector and a norm is log2(G) shuffles.  A warp takes
 // one row (or a share of its heads when there are few rows) and computes the row's sines once for
-// all heads.  The backward sweeps the query heads of its rows, then the key heads, so that a thread
-// holds one gain and one gain gradient, and what it will read is on its way three turns ahead, by
-// asynchronous copies into slots of shared memory that no other thread touches: with plain loads,
-// registers limited what was in flight (115 us instead of 90 below).  In the forward four heads' plain
-// loads per turn do as well (61 us; the queue 64).
+// all heads.  In the backward what a thread will read is on its way three turns ahead, by asynchronous
+// copies into slots of shared memory that no other thread touches: with plain loads, registers limited
+// what was in flight (115 us instead of 89 below).  In the forward four heads' plain loads per turn do
+// as well (61 us; the queue 64).
 //
 // B200, 16384 rows of 32 + 8 heads of 128, bf16: forward 61 us (5.5 TB/s, 84% of the copy rate),
-// backward 90 us (5.6 TB/s, 85%), the gains' sum included.
+// backward 89 us (5.7 TB/s, 87%), the gains' sum included.
 #include <cuda_runtime.h>
 #include <math.h>
 
@@ -81,25 +80,28 @@ __device__ __forceinline__ void copy_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
 }
 
-// What a thread reads in its coming turns: MATS matrices' two vectors of a head each, for `depth` turns.
-// Slots are [turn][vector part][thread]; fetch() is called once per turn and asks for the next one.
-template <class T, int MATS, int DEPTH>
+// What a thread reads in its coming turns: the two vectors of a head of x and of dy each, DEPTH turns
+// ahead.  A row is turns_q turns over the query heads, then turns_k over the key heads, `slots` heads a
+// turn.  Slots are [turn][vector part][thread]; fetch() is called once per turn and asks for the next one.
+template <class T, int DEPTH>
 struct HeadQueue {
-  static constexpr int Q = sizeof(Raw8<T>) / 16, PARTS = 2 * MATS * Q;
-  uint4* slots;
-  const T* base[MATS];
-  long ld[MATS];
+  static constexpr int Q = sizeof(Raw8<T>) / 16, PARTS = 4 * Q;
+  uint4* mem;
+  const T* base[2];
+  long ld[2];
   long row, rows, row_step;
-  int turn, turns, head, head_step, heads, half, hd, stage;
+  int turn, turns_q, turns_k, slot, slots, H, HK, half, hd, stage;
   bool on;
 
   __device__ __forceinline__ void fetch() {
     if (row < rows) {
-      if (on && head < heads) {
-        uint4* c = slots + stage * PARTS * kWarps * 32;
+      const bool key = turn >= turns_q;
+      const int h = (key ? turn - turns_q : turn) * slots + slot;
+      if (on && h < (key ? HK : H)) {
+        uint4* c = mem + stage * PARTS * kWarps * 32;
 #pragma unroll
-        for (int m = 0; m < MATS; ++m) {
-          const T* p = base[m] + row * ld[m] + (long)head * hd;
+        for (int m = 0; m < 2; ++m) {
+          const T* p = base[m] + row * ld[m] + (long)(h + (key ? H : 0)) * hd;
 #pragma unroll
           for (int q = 0; q < Q; ++q) {
             copy_async16(c + (m * 2 * Q + q) * kWarps * 32, (const char*)p + 16 * q);
@@ -107,10 +109,8 @@ struct HeadQueue {
           }
         }
       }
-      head += head_step;
-      if (++turn == turns) {
+      if (++turn == turns_q + turns_k) {
         turn = 0;
-        head -= turns * head_step;
         row += row_step;
       }
     }
@@ -119,7 +119,7 @@ struct HeadQueue {
   }
   // The oldest turn's vectors; its slots are the next fetch()'s.
   __device__ __forceinline__ void read(int m, Raw8<T>& a, Raw8<T>& b) const {
-    const uint4* c = slots + (stage * PARTS + m * 2 * Q) * kWarps * 32;
+    const uint4* c = mem + (stage * PARTS + m * 2 * Q) * kWarps * 32;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       a.q[q] = c[q * kWarps * 32];
@@ -219,10 +219,9 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm)
   __shared__ double freq[kMaxHalf];
   __shared__ float cs_all[kWarps][kMaxHalf], sn_all[kWarps][kMaxHalf];
   __shared__ float red[kWarps][2 * kMaxHalf];
+  __shared__ float4 key_acc_all[4 * kWarps * 32];  // the key gain's gradient; the query gain's is in registers
   const int half = hd >> 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < half; i += blockDim.x) freq[i] = turns_per_position(turns, i);
-  __syncthreads();
   const int d = (lane % G) * 8;
   const bool on = d < half;
   const int slots = (32 / G) * warps_per_row;
@@ -230,33 +229,38 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm)
   const int rows_per_block = kWarps / warps_per_row;
   const long row0 = (long)blockIdx.x * rows_per_block + warp / warps_per_row, row_step = (long)gridDim.x * rows_per_block;
   const float inv_n = 1.0f / (float)hd;
-#pragma unroll 1
-  for (int part = 0; part < 2; ++part) {
-    const int n = part ? HK : H, its = (n + slots - 1) / slots;
-    const long first = (part ? (long)H * hd : 0) + d;
-    HeadQueue<T, 2, DEPTH> queue{ring + threadIdx.x, {x + first, dy + first}, {ldx, lddy}, row0, n ? rows : 0, row_step,
-                                 0, its, slot, slots, n, half, hd, 0, on};
+  HeadQueue<T, DEPTH> queue{ring + threadIdx.x, {x + d, dy + d}, {ldx, lddy}, row0, rows, row_step, 0,
+                            (H + slots - 1) / slots, (HK + slots - 1) / slots, slot, slots, H, HK, half, hd, 0, on};
 #pragma unroll
-    for (int k = 0; k < DEPTH; ++k) queue.fetch();
-    float ga[8], gb[8], acc[16];
+  for (int k = 0; k < DEPTH; ++k) queue.fetch();
+  for (int i = threadIdx.x; i < half; i += blockDim.x) freq[i] = turns_per_position(turns, i);
+  __syncthreads();
+  float acc[16];
+  float4* const key_acc = key_acc_all + threadIdx.x;  // 4 of them, kWarps * 32 apart
+#pragma unroll
+  for (int j = 0; j < 16; ++j) acc[j] = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) key_acc[j * kWarps * 32] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (long row = row0; row < rows; row += row_step) {
+    row_turns(freq, cs_all[warp], sn_all[warp], half, (int)(row % S), lane);
+    float cs[8], sn[8];
     if (on) {
-      load8((part ? gk : gq) + d, ga);
-      load8((part ? gk : gq) + half + d, gb);
-    }
 #pragma unroll
-    for (int j = 0; j < 16; ++j) acc[j] = 0.f;
-    for (long row = row0; row < rows && n; row += row_step) {
-      row_turns(freq, cs_all[warp], sn_all[warp], half, (int)(row % S), lane);
-      float cs[8], sn[8];
-      if (on) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          cs[j] = cs_all[warp][d + j];
-          sn[j] = sn_all[warp][d + j];
-        }
+      for (int j = 0; j < 8; ++j) {
+        cs[j] = cs_all[warp][d + j];
+        sn[j] = sn_all[warp][d + j];
       }
-      T* dxr = dx + row * lddx + first;
-      for (int h = slot; h < its * slots; h += slots) {
+    }
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {
+      const int n = part ? HK : H;
+      T* dxr = dx + row * lddx + (part ? (long)H * hd : 0) + d;
+      float ga[8], gb[8];
+      if (on) {
+        load8((part ? gk : gq) + d, ga);
+        load8((part ? gk : gq) + half + d, gb);
+      }
+      for (int h = slot; h - slot < n; h += slots) {
         copy_async_wait<DEPTH - 1>();
         const bool mine = on && h < n;
         float a[8], b[8], va[8], vb[8], ss = 0.f, dot = 0.f;
@@ -282,21 +286,52 @@ __global__ void __launch_bounds__(kWarps * 32, kPerSm)
         __syncwarp();
         queue.fetch();
         if (mine) {
-          float o1[8], o2[8];
+          float o1[8], o2[8], g1[8], g2[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const float wa = va[j] * r, wb = vb[j] * r;
-            acc[j] += wa * a[j];
-            acc[8 + j] += wb * b[j];
+            g1[j] = wa * a[j];
+            g2[j] = wb * b[j];
             o1[j] = wa * ga[j] - a[j] * (m * r);
             o2[j] = wb * gb[j] - b[j] * (m * r);
           }
           store8(dxr + (long)h * hd, o1);
           store8(dxr + (long)h * hd + half, o2);
+          if (part == 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              acc[j] += g1[j];
+              acc[8 + j] += g2[j];
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float* g = j < 2 ? g1 + 4 * j : g2 + 4 * (j - 2);
+              float4 v = key_acc[j * kWarps * 32];
+              v.x += g[0];
+              v.y += g[1];
+              v.z += g[2];
+              v.w += g[3];
+              key_acc[j * kWarps * 32] = v;
+            }
+          }
         }
       }
     }
-    copy_async_wait<0>();
+  }
+  copy_async_wait<0>();
+#pragma unroll 1
+  for (int part = 0; part < 2; ++part) {
+    if (part) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 v = key_acc[j * kWarps * 32];
+        acc[4 * j] = v.x;
+        acc[4 * j + 1] = v.y;
+        acc[4 * j + 2] = v.z;
+        acc[4 * j + 3] = v.w;
+      }
+    }
     // lanes that hold the same columns, then the block's warps, in a fixed order
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
@@ -352,7 +387,7 @@ Turns turns_of(int hd, double theta) {
 }
 
 // Warps that share a row's heads: one (a row's sines are computed by each), unless the rows fill less than
-// half of the GPU's warps with one each.  1000 rows of 32 + 8 heads of 128, forward / backward: 6.9 / 13.7 us
+// half of the GPU's warps with one each.  1000 rows of 32 + 8 heads of 128, forward / backward: 6.9 / 13.0 us
 // with this limit of 8 warps per SM, 7.5 / 15.8 with 16, 10.3 / 19.1 with 32.
 int warps_per_row_of(int rows, int heads, int slots, int sms) {
   int w = 1;
