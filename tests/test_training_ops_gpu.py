@@ -102,6 +102,27 @@ def test_qk_norm_rope_far_positions():
     oracle.close(y[rows], want, 32 * oracle.U * torch.cat([a.abs() + b.abs()] * 2, 1))
 
 
+def test_qk_norm_rope_past_2_to_the_31_elements():
+    T, H, HK, hd = 360_000, 32, 8, 128
+    qkv = torch.ones(T, (H + 2 * HK) * hd, dtype=torch.bfloat16, device=DEV)
+    qkv[-3:] = _rand(3, qkv.shape[1], dtype=torch.bfloat16)
+    g = _rand(hd, dtype=torch.bfloat16)
+    shape = (3, H, HK, hd, 10000.0)  # 360000 is a multiple of 3: the last rows have positions 0, 1, 2
+    y = ops.qk_norm_rope(qkv, g, g, *shape)
+    oracle.close(y[-3:], *oracle.heads_forward(qkv[-3:], g, g, *shape, 1e-5))
+    del y
+    dy = torch.zeros_like(qkv)
+    dy[-3:] = _rand(3, qkv.shape[1], dtype=torch.bfloat16)
+    tail = dy[-3:].clone()
+    dg = torch.zeros(2, hd, device=DEV)
+    ops.qk_norm_rope_bwd(dy, qkv, g, g, *shape, dg[0], dg[1], out=dy)
+    want = oracle.heads_backward(tail, qkv[-3:], g, g, *shape, 1e-5)
+    oracle.close(dy[-3:, :(H + HK) * hd], *want[0], "dx")
+    oracle.close(dg[0], *want[1], "dq_gain")  # the other rows' gradients are zero
+    oracle.close(dg[1], *want[2], "dk_gain")
+    assert dy[:-3, :(H + HK) * hd].count_nonzero() == 0
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_qk_norm_rope_layouts(dtype):
     """Rows on no 16-byte boundary, a wide row stride, a transposed layout and gains inside a larger buffer."""
@@ -200,7 +221,10 @@ def test_dropout_captured_graph_draws_a_new_mask_each_replay():
 
 # ------------------------------------------------------------------ losses over logits
 
-LOGITS = [(1, 1), (2, 7), (5, 8), (33, 100), (64, 1024), (37, 5003), (9, 16391), (16, 50257), (3, 128256), (2, 300007)]
+# Few rows of every width: a warp, a block, a cluster of 2, 4 or 8 blocks per row, and past what a cluster holds;
+# then many rows: 4 warps per row, and each block size of the stream kernels, several rows to a block.
+LOGITS = [(1, 1), (2, 7), (5, 8), (33, 100), (64, 1024), (100, 3001), (37, 5003), (9, 16391), (16, 50257), (3, 128256),
+          (2, 300007), (400, 1025), (1500, 4096), (3100, 4099), (2000, 12345), (1100, 30011), (700, 60001), (400, 131075)]
 
 
 def _logits(T, V, dtype):
@@ -232,8 +256,10 @@ def test_token_logprobs(T, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("V", [13, 64, 5003, 50257, 128256])
-def test_rows_of_infinities_and_nan(V, dtype):
+@pytest.mark.parametrize("V,copies", [(13, 1), (64, 1), (5003, 1), (50257, 1), (128256, 1), (2051, 40), (5003, 200),
+                                      (29000, 80), (61003, 50), (120007, 40)])
+def test_rows_of_infinities_and_nan(V, copies, dtype):
+    """``copies`` of eight rows: the last eight, which blocks with several rows reach, are looked at."""
     x = _rand(8, (V + 7) // 8 * 8, dtype=dtype, scale=2.0)
     low = torch.finfo(dtype).min
     x[0] = -math.inf                 # nothing left
@@ -244,7 +270,12 @@ def test_rows_of_infinities_and_nan(V, dtype):
     x[5] = low                       # every logit the lowest value: a uniform row
     x[6, :V - 1] = -math.inf         # one value left, the last
     t = torch.tensor([2, 1, 0, 0, 0, 5, V - 1, 7], device=DEV)
-    lp, stats = ops.token_logprobs(x, V, t)
+    many = lambda v: v.repeat(copies, *[1] * (v.dim() - 1))  # noqa: E731
+    last = lambda v: v[-8:]  # noqa: E731
+    xs, ts = many(x), many(t)
+    lps, all_stats = ops.token_logprobs(xs, V, ts)
+    lp, stats = last(lps), last(all_stats)
+    assert torch.equal(lps.nan_to_num(7.0), many(lp).nan_to_num(7.0))
     (want, slack), (wstats, sslack), _, _ = oracle.logprobs(x, V, t)
     fine = [1, 4, 5, 6, 7]
     oracle.close(lp[fine], want[fine], slack[fine], "logp")
@@ -252,20 +283,19 @@ def test_rows_of_infinities_and_nan(V, dtype):
     assert lp[0] == -math.inf and stats[0].tolist() == [-math.inf, 0.0]
     assert lp[2].isnan() and stats[2, 1].isnan() and lp[3].isnan()
     up = torch.ones(8, device=DEV)
-    d = ops.token_logprobs_bwd(x, V, t, stats, up)
+    d = last(ops.token_logprobs_bwd(xs, V, ts, all_stats, many(up)))
     assert d[0].eq(0).all() and d[1, 3:].eq(0).all() and d[2].isnan().all()
     oracle.close(d[fine], *[v[fine] for v in oracle.dlogits(x, V, t, up)], "dlogits")
     assert ops.token_logprobs_bwd(x, V, t, stats, torch.zeros(8, device=DEV)).eq(0).all()
     # the one-pass loss on the same rows
-    rows = (8,)
-    z, one = torch.zeros(rows, device=DEV), torch.ones(rows, device=DEV)
+    z, one = torch.zeros(8, device=DEV), torch.ones(8, device=DEV)
     w = one.clone()
     w[[0, 2, 3]] = 0
     old = torch.where(w > 0, lp, math.nan)
-    loss, lp2, d = ops.policy_loss_chunk(x, V, t, old, one, w)
+    loss, lp2, d = map(last, ops.policy_loss_chunk(xs, V, ts, many(old), many(one), many(w)))
     assert loss[[0, 2, 3]].eq(0).all() and d[[0, 2, 3]].eq(0).all() and lp2[0] == -math.inf
     assert torch.allclose(loss[fine], -one[fine], atol=1e-5) and d[fine].isfinite().all()
-    loss, _, d = ops.policy_loss_chunk(x, V, t, z, one, z)
+    loss, _, d = ops.policy_loss_chunk(xs, V, ts, many(z), many(one), many(z))
     assert loss.eq(0).all() and d.eq(0).all()
 
 
@@ -340,7 +370,7 @@ def test_logits_past_2_to_the_31_elements():
 
 
 @pytest.mark.parametrize("form,smoothing", [("sigmoid", 0.0), ("sigmoid", 0.1), ("squared", 0.0)])
-@pytest.mark.parametrize("P,S", [(1, 1), (2, 7), (3, 300), (5, 4097), (1, 200_003), (200, 33), (0, 4), (2, 0)])
+@pytest.mark.parametrize("P,S", [(1, 1), (2, 7), (3, 300), (5, 4097), (20, 17001), (1, 200_003), (200, 33), (0, 4), (2, 0)])
 def test_preference_loss(P, S, form, smoothing):
     lp, ref = -5 * torch.rand(2 * P, S, device=DEV), -5 * torch.rand(2 * P, S, device=DEV)
     mask = torch.rand(2 * P, S, device=DEV) < 0.7
@@ -396,6 +426,28 @@ def test_preference_step_on_a_side_stream_and_captured():
     torch.cuda.synchronize()
     for _, res in graphs:
         for a, b in zip(res, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T,V", [(30, 50257), (300, 50257), (200, 500)])  # a cluster, a stream and a warp per row
+def test_policy_loss_captured_and_on_two_streams(T, V):
+    x, t = _logits(T, V, torch.bfloat16)
+    old, adv = -9 + _rand(T), _rand(T)
+    want = [v.clone() for v in ops.policy_loss_chunk(x, V, t, old, adv)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = ops.policy_loss_chunk(x, V, t, old, adv)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(3):
+        for s in streams:  # two eager calls and a replay under way at once
+            with torch.cuda.stream(s):
+                outs.append(ops.policy_loss_chunk(x, V, t, old, adv))
+        graph.replay()
+    torch.cuda.synchronize()
+    for got in outs + [res]:
+        for a, b in zip(got, want):
             assert torch.equal(a, b)
 
 

@@ -10,16 +10,21 @@ import numpy as np
 import torch
 
 U = 2.0 ** -24  # half a step of fp32
+WORK = "cuda" if torch.cuda.is_available() else "cpu"  # where the 64-bit arithmetic runs
+
+
+def w64(t):
+    return t.detach().to(WORK).double()
 
 
 def close(got, ref, slack, what=""):
     """|got - ref| <= half a step of got's type at ref, plus slack; equal NaN and infinities."""
     info = torch.finfo(got.dtype)
-    g, r = got.detach().cpu().double(), ref.cpu().double()
+    g, r = w64(got), w64(ref)
     assert g.shape == r.shape, (what, g.shape, r.shape)
     odd = ~torch.isfinite(r)
     assert torch.equal(g[odd].nan_to_num(0.5), r[odd].nan_to_num(0.5)), f"{what}: infinities or NaN differ"
-    bound = r.abs() * (info.eps / 2) + info.smallest_normal * info.eps / 2 + slack.cpu().double()
+    bound = r.abs() * (info.eps / 2) + info.smallest_normal * info.eps / 2 + w64(slack)
     bad = ((g - r).abs() > bound) & ~odd | (~torch.isfinite(g) & ~odd)
     if bad.any():
         i = tuple(torch.nonzero(bad)[0].tolist())
@@ -30,16 +35,16 @@ def close(got, ref, slack, what=""):
 # ------------------------------------------------------------------ head norms and rotation
 
 def _rotation(rows, seq, hd, theta):
-    pos = torch.arange(rows, dtype=torch.float64) % seq
-    freq = torch.exp(torch.arange(hd // 2, dtype=torch.float64) * (-2.0 * math.log(theta) / hd))
+    pos = torch.arange(rows, dtype=torch.float64, device=WORK) % seq
+    freq = torch.exp(torch.arange(hd // 2, dtype=torch.float64, device=WORK) * (-2.0 * math.log(theta) / hd))
     ang = torch.outer(pos, freq)
     return ang.cos()[:, None], ang.sin()[:, None]
 
 
 def heads_forward(qkv, gq, gk, seq, H, HK, hd, theta, eps):
     T = qkv.shape[0]
-    x = qkv[:, :(H + HK) * hd].cpu().double().view(T, H + HK, hd)
-    g = torch.cat([gq.cpu().double().expand(H, -1), gk.cpu().double().expand(HK, -1)])
+    x = w64(qkv[:, :(H + HK) * hd]).view(T, H + HK, hd)
+    g = torch.cat([w64(gq).expand(H, -1), w64(gk).expand(HK, -1)])
     u = x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) * g
     cs, sn = _rotation(T, seq, hd, theta)
     a, b = u[..., :hd // 2], u[..., hd // 2:]
@@ -52,9 +57,9 @@ def heads_forward(qkv, gq, gk, seq, H, HK, hd, theta, eps):
 def heads_backward(dqk, qkv, gq, gk, seq, H, HK, hd, theta, eps):
     """((dx, slack), (dq_gain, slack), (dk_gain, slack))"""
     T = qkv.shape[0]
-    x = qkv[:, :(H + HK) * hd].cpu().double().view(T, H + HK, hd)
-    dy = dqk[:, :(H + HK) * hd].cpu().double().view(T, H + HK, hd)
-    g = torch.cat([gq.cpu().double().expand(H, -1), gk.cpu().double().expand(HK, -1)])
+    x = w64(qkv[:, :(H + HK) * hd]).view(T, H + HK, hd)
+    dy = w64(dqk[:, :(H + HK) * hd]).view(T, H + HK, hd)
+    g = torch.cat([w64(gq).expand(H, -1), w64(gk).expand(HK, -1)])
     cs, sn = _rotation(T, seq, hd, theta)
     a, b = dy[..., :hd // 2], dy[..., hd // 2:]
     du = torch.cat([a * cs + b * sn, b * cs - a * sn], -1)
@@ -89,9 +94,9 @@ def keep_bits(n, seed, offset):
 
 def dropout(x, p, seed, offset, residual=None):
     cut = round(p * 65536)
-    keep = torch.from_numpy((keep_bits(x.numel(), seed, offset) >= cut).reshape(x.shape))
-    y = torch.where(keep, x.cpu().double() * 65536 / (65536 - cut), 0.0)
-    r = torch.zeros_like(y) if residual is None else residual.cpu().double()
+    keep = torch.from_numpy((keep_bits(x.numel(), seed, offset) >= cut).reshape(x.shape)).to(WORK)
+    y = torch.where(keep, w64(x) * 65536 / (65536 - cut), 0.0)
+    r = torch.zeros_like(y) if residual is None else w64(residual)
     return y + r, 2 * U * y.abs() + (0 if residual is None else U * (y.abs() + r.abs())), keep
 
 
@@ -99,8 +104,8 @@ def dropout(x, p, seed, offset, residual=None):
 
 def logprobs(logits, vocab, targets):
     """((logps, slack), (stats, slack), softmax, valid) in 64 bits; stats are [T, 2], a row's maximum and its sum."""
-    x = logits[:, :vocab].cpu().double()
-    t = targets.cpu()
+    x = w64(logits[:, :vocab])
+    t = targets.to(WORK)
     valid = (t >= 0) & (t < vocab)
     m = x.nan_to_num(nan=-math.inf, posinf=math.inf, neginf=-math.inf).amax(-1, keepdim=True)
     e = torch.exp(x - torch.where(m == -math.inf, 0.0, m))
@@ -118,11 +123,11 @@ def logprobs(logits, vocab, targets):
 
 def dlogits(logits, vocab, targets, dlogps, dslack=0.0):
     (_, ls), (stats, _), p, valid = logprobs(logits, vocab, targets)
-    up = torch.where(valid, dlogps.cpu().double(), 0.0)
-    hot = torch.zeros_like(p).scatter_(1, targets.cpu().clamp(0, vocab - 1)[:, None], 1.0)
+    up = torch.where(valid, w64(dlogps), 0.0)
+    hot = torch.zeros_like(p).scatter_(1, targets.to(WORK).clamp(0, vocab - 1)[:, None], 1.0)
     zero = (up == 0)[:, None]
     d = torch.where(zero, 0.0, (hot - p) * up[:, None])
-    x = logits[:, :vocab].cpu().double()
+    x = w64(logits[:, :vocab])
     # the exponential's own steps, and those of the sum
     far = (x - stats[:, :1]).abs().nan_to_num(0.0, 0.0, 0.0)
     rel = 2 * (2 + 1.2 * far) * U + ls[:, None]
@@ -133,16 +138,16 @@ def dlogits(logits, vocab, targets, dlogps, dslack=0.0):
 def policy(logits, vocab, targets, old, adv, w, ref, low, high, kl, scale):
     """((losses, slack), (logps, slack), (dlogits, slack))"""
     (lp, ls), _, _, valid = logprobs(logits, vocab, targets)
-    tg = targets.cpu()
+    tg = targets.to(WORK)
     has = (tg >= 0) & (tg < vocab)
-    w = torch.ones_like(lp) if w is None else w.cpu().double()
-    A, ratio = adv.cpu().double(), torch.exp(lp - old.cpu().double())
+    w = torch.ones_like(lp) if w is None else w64(w)
+    A, ratio = w64(adv), torch.exp(lp - w64(old))
     gained = torch.where(A >= 0, A * ratio.clamp(max=1 + high), A * ratio.clamp(min=1 - low))
     inside = torch.where(A >= 0, ratio <= 1 + high, ratio >= 1 - low)
     loss, d = -gained, -torch.where(inside, A * ratio, 0.0)
     big = A.abs() * ratio.clamp(min=1)
     if ref is not None and kl:
-        back = ref.cpu().double() - lp
+        back = w64(ref) - lp
         loss, d = loss + kl * (torch.exp(back) - 1 - back), d + kl * (1 - torch.exp(back))
         big = big + kl * (torch.exp(back) + 1)
     used = has & (w != 0)
@@ -154,8 +159,8 @@ def policy(logits, vocab, targets, old, adv, w, ref, low, high, kl, scale):
 
 def preference(logps, ref, mask, beta, form, smoothing, scale):
     """(losses, rewards, dlogps): fp64 inside, so their slack is nothing but the last rounding."""
-    m = mask.cpu()
-    diff = torch.where(m, logps.cpu().double() - ref.cpu().double(), 0.0)
+    m = mask.to(WORK)
+    diff = torch.where(m, w64(logps) - w64(ref), 0.0)
     r, n = diff.sum(1), m.sum(1).clamp(min=1)
     c, j = r[0::2], r[1::2]
     if form == "sigmoid":

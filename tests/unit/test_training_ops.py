@@ -147,7 +147,7 @@ POLICY = dict(low=0.2, high=0.3, kl=0.05, scale=0.5)
 
 def _policy_inputs(x, V, t, device="cpu"):
     T = t.shape[0]
-    lp = oracle.logprobs(x, V, t)[0][0].float()
+    lp = oracle.logprobs(x, V, t)[0][0].float().cpu()
     r = torch.randn(T) * 0.2
     r[::3] = 0.0  # unchanged policy: both sides of the max equal
     old, ref, adv = lp - r, lp + torch.randn(T) * 0.1, torch.randn(T)
