@@ -260,6 +260,7 @@ int dtype_code(const Tensor& t, const char* name) {
   }
   return -1;
 }
+constexpr int64_t kMostRows = int64_t(1) << 30;  // the kernels' row and column indexes are 32-bit
 bool aligned16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
 // Rows the kernels read and write in place: unit column stride, 16-byte aligned, a leading dimension
 // that is a multiple of 8.
@@ -276,7 +277,7 @@ Tensor as_rows(const Tensor& t, const char* name, const Tensor& like, int64_t ro
   TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == rows && t.size(1) >= cols && t.scalar_type() == like.scalar_type() &&
                         t.device() == like.device(),
                     name, " must be [", rows, ", >= ", cols, "] ", like.scalar_type(), " on ", like.device());
-  TORCH_CHECK_VALUE(rows < INT32_MAX && cols < INT32_MAX, name, " is too large");
+  TORCH_CHECK_VALUE(rows <= kMostRows && cols <= kMostRows, name, " is larger than 2^30 rows or columns");
   if (is_rows(t)) return t;
   Tensor copy = padded_rows(like, rows, cols);
   copy.copy_(t.narrow(1, 0, cols));
@@ -490,7 +491,7 @@ std::tuple<Tensor, Tensor, Tensor> preference_loss(const Tensor& logps, const Te
                                                    double beta, double label_smoothing, bool squared,
                                                    double grad_scale) {
   TORCH_CHECK_VALUE(logps.is_cuda() && logps.dim() == 2 && logps.size(0) % 2 == 0 &&
-                        logps.scalar_type() == at::kFloat && logps.size(1) < INT32_MAX && logps.size(0) < INT32_MAX,
+                        logps.scalar_type() == at::kFloat && logps.size(1) <= kMostRows && logps.size(0) <= kMostRows,
                     "preference_loss: logps must be fp32 [2 pairs, S]");
   TORCH_CHECK_VALUE(beta > 0 && label_smoothing >= 0 && label_smoothing <= 1,
                     "preference_loss: needs beta > 0 and 0 <= label_smoothing <= 1");

@@ -5,8 +5,8 @@
 // d logp / d x_c = [c = t] - exp(x_c - m) / s.  The pair (m, s) is what the backward gets: beside a
 // logit of the type's lowest value a log-sum-exp could not hold log s.  A target outside [0, V) marks
 // a row without a token: logp 0, gradient 0.  Logits of -inf have probability 0; a row of nothing but
-// -inf has m = logp = -inf, s = 0 and gradient 0.  NaN and +inf propagate within their row, unless the row's weight (or upstream
-// gradient) is 0: such a row's gradient is 0 whatever it holds.
+// -inf has m = logp = -inf, s = 0 and gradient 0.  NaN and +inf propagate within their row, unless the
+// row's weight (or upstream gradient) is 0: such a row's gradient is 0 whatever it holds.
 //
 // Sums are fp32; logp is formed in fp64 from the fp32 maximum and sum, so that it carries one rounding.
 // Exponentials are ex2 of (x - m) log2(e) with the constant in two parts: with one fp32 constant every
@@ -985,7 +985,7 @@ int dispatch_rows(const RowArgs& a, cudaStream_t s) {
   // blocks per row that hold it in registers, and more of them while the rows leave half of the GPU
   // idle and every block keeps 2048 columns
   int need = 1;
-  while (V > need * 512 * per_thread) need *= 2;
+  while (need <= 8 && V > need * 512 * per_thread) need *= 2;
   if (a.rows > sms || need > 8) {
     if constexpr (!POLICY) {
       // 128 / 256 / 512 threads: V = 50257 (8192 rows) 184 / 141 / 159 us, 128256 (4096 rows) 224 / 171 / 171

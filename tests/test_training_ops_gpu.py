@@ -45,6 +45,8 @@ def test_refusals():
         ops.token_logprobs_bwd(torch.zeros(4, 96, device=DEV), 96, t, st, v, out=torch.zeros(4, 97, device=DEV))
     with pytest.raises(ValueError):
         ops.dropout(flat[:64], 0.1, 0, 0, out=flat[65:129])
+    with pytest.raises(ValueError):  # more columns than 32-bit indexes take
+        ops.token_logprobs(torch.zeros(1, 1, device=DEV).expand(1, (1 << 30) + 8), (1 << 30) + 1, t[:1])
     with pytest.raises(ValueError):  # another device
         ops.token_logprobs(torch.zeros(4, 96, device=DEV), 96, t.cpu())
 
