@@ -22,6 +22,8 @@ from dataclasses import dataclass
 import torch
 from torch import nn
 
+from meshtrain_b200 import ops
+
 
 def layer_seed(seed: int, index: int) -> int:
     return (seed * 1_000_003 + index * 7919) % (2**31 - 1)
@@ -29,6 +31,7 @@ def layer_seed(seed: int, index: int) -> int:
 
 RNG_KEY = "rng"  # saved[RNG_KEY]: (seed, offset) of a layer's random numbers in this pass
 RNG_SITES = 4    # offsets a layer may use from that one on
+DROPPED = "dropped"  # saved[DROPPED]: the probability a pass dropped with; absent if it did not
 
 
 class PipelineLayer(nn.Module):
@@ -55,6 +58,15 @@ class PipelineLayer(nn.Module):
             saved[RNG_KEY] = (seed, base * RNG_SITES % 2**62)
         seed, offset = saved[RNG_KEY]
         return seed, offset + site
+
+    def _drop(self, x: torch.Tensor, saved: dict, site: int, residual: torch.Tensor | None = None) -> torch.Tensor:
+        """``residual`` + dropout(x), in x's memory."""
+        saved[DROPPED] = self.dropout
+        return ops.dropout(x, self.dropout, *self._rng(saved, site), residual=residual, out=x)
+
+    def _drop_grad(self, dy: torch.Tensor, saved: dict, site: int) -> torch.Tensor:
+        """Gradient of what that pass dropped from, whatever mode the layer is in by now."""
+        return ops.dropout(dy, saved[DROPPED], *self._rng(saved, site)) if DROPPED in saved else dy
 
     def fwd(self, x: torch.Tensor, saved: dict) -> torch.Tensor:  # pragma: no cover - abstract
         raise NotImplementedError

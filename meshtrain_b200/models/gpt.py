@@ -49,15 +49,14 @@ class Embedding(PipelineLayer):
         B, S = tokens.shape
         out = ops.embedding(tokens, self.tok.weight, None if self.pos is None else self.pos.weight, S)
         if self.dropping():
-            out = ops.dropout(out, self.dropout, *self._rng(saved, 2), out=out)
+            out = self._drop(out, saved, 2)
         saved["ids"] = tokens
         return out.view(B, S, -1)
 
     def bwd(self, dy, saved, grads):
         ids = saved["ids"]
         S = ids.shape[1]
-        if self.dropping():
-            dy = ops.dropout(dy, self.dropout, *self._rng(saved, 2))
+        dy = self._drop_grad(dy, saved, 2)
         ops.embedding_bwd_(ids, dy, grads["tok.weight"], grads.get("pos.weight"), S)
         return None
 
@@ -92,12 +91,7 @@ class Block(PipelineLayer):
         one pass over its output."""
         if not self.dropping():
             return ops.linear(y, lin.weight, lin.bias, residual=residual)
-        h = ops.linear(y, lin.weight, lin.bias)
-        return ops.dropout(h, self.dropout, *self._rng(saved, site), residual=residual, out=h)
-
-    def _branch_grad(self, dy, saved, site):
-        """Gradient of that branch's linear output."""
-        return ops.dropout(dy, self.dropout, *self._rng(saved, site)) if self.dropping() else dy
+        return self._drop(ops.linear(y, lin.weight, lin.bias), saved, site, residual)
 
     # The block is two residual halves; each half is also usable as a pipeline
     # layer of its own (models/split.py), so a stage boundary may fall between them.
@@ -130,7 +124,7 @@ class Block(PipelineLayer):
     def mlp_bwd(self, dy, saved, grads):
         B, S, d = saved["shape"]
         dy2 = dy.reshape(B * S, d)
-        db = self._branch_grad(dy2, saved, 1)
+        db = self._drop_grad(dy2, saved, 1)
         dh = ops.linear_dgrad(db, self.fc2.weight, gelu_pre=saved["h"])
         ops.linear_wgrad_(db, saved["g"], grads["fc2.weight"], grads["fc2.bias"])
         del db
@@ -147,7 +141,7 @@ class Block(PipelineLayer):
         hd = d // H
         T = B * S
         dx1 = dy.reshape(T, d)
-        db = self._branch_grad(dx1, saved, 0)
+        db = self._drop_grad(dx1, saved, 0)
         do = ops.linear_dgrad(db, self.proj.weight)
         ops.linear_wgrad_(db, saved["o"].reshape(T, d), grads["proj.weight"], grads["proj.bias"])
         del db

@@ -62,7 +62,7 @@ class LlamaBlock(PipelineLayer):
         v = qkv[:, (H + Hk) * hd:].view(B, S, Hk, hd)
         return q, k, v
 
-    _branch, _branch_grad = Block._branch, Block._branch_grad
+    _branch = Block._branch
 
     # Two residual halves, each usable as a pipeline layer of its own (models/split.py).
     HALVES = (("attn_norm", "wqkv", "wo"), ("mlp_norm", "w_gate_up", "w_down"))
@@ -97,7 +97,7 @@ class LlamaBlock(PipelineLayer):
     def mlp_bwd(self, dy, saved, grads):
         B, S, d = saved["shape"]
         dy2 = dy.reshape(B * S, d)
-        db = self._branch_grad(dy2, saved, 1)
+        db = self._drop_grad(dy2, saved, 1)
         dact = ops.linear_dgrad(db, self.w_down.weight)
         ops.linear_wgrad_(db, saved["act"], grads["w_down.weight"])
         del db
@@ -114,7 +114,7 @@ class LlamaBlock(PipelineLayer):
         T = B * S
         H, Hk, hd = self.n_heads, self.n_kv_heads, self.head_dim
         dx1 = dy.reshape(T, d)
-        db = self._branch_grad(dx1, saved, 0)
+        db = self._drop_grad(dx1, saved, 0)
         do = ops.linear_dgrad(db, self.wo.weight)
         ops.linear_wgrad_(db, saved["o"].reshape(T, d), grads["wo.weight"])
         del db

@@ -221,6 +221,26 @@ def test_layers_under_autograd_drop_alike_both_ways(cfg):
     assert torch.equal(y, y2) and torch.equal(x.grad, dx)
 
 
+@pytest.mark.parametrize("index", [0, 1])
+@pytest.mark.parametrize("train", [True, False])
+def test_backward_follows_its_forward_after_a_change_of_mode(index, train):
+    """The gradient is that of the pass that ran: a layer put into the other mode before its backward runs
+    changes nothing."""
+    spec = build_model_spec(CFGS[0], seed=1)
+    layer = spec.build_layer(index).train(train)
+    x = torch.randint(0, 61, (2, 12)) if index == 0 else torch.randn(2, 12, 32)
+    dy = torch.randn(2, 12, 32)
+    out = []
+    for change in (False, True):
+        saved = {RNG_KEY: (7, 16)}
+        grads = {n: torch.zeros_like(q) for n, q in layer.named_parameters()}
+        with torch.no_grad():
+            layer.train(train).fwd(x, saved)
+            dx = layer.train(train != change).bwd(dy, saved, grads)
+        out.append([*grads.values()] + ([] if dx is None else [dx]))
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
 def _pair_inputs(spec, B=4):
     x, y = spec.make_batch(0, B)
     y = y.clone()
