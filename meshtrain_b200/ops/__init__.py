@@ -806,7 +806,9 @@ def preference_loss(logps: torch.Tensor, ref_logps: torch.Tensor, mask: torch.Te
     r0, r1 = r[0::2], r[1::2]
     if form == "sigmoid":
         h = beta * (r0 - r1)
-        losses = -(1 - label_smoothing) * F.logsigmoid(h) - label_smoothing * F.logsigmoid(-h)
+        # a side of weight 0 is left out: it may be infinite
+        losses = sum((-w * F.logsigmoid(g) for w, g in ((1 - label_smoothing, h), (label_smoothing, -h)) if w),
+                     torch.zeros_like(h))
         up = beta * (label_smoothing - torch.sigmoid(-h))
         up = torch.stack([up, -up], -1).reshape(-1)
     else:

@@ -869,7 +869,8 @@ __global__ void __launch_bounds__(NT) preference_kernel(PreferenceArgs a) {
   } else {
     const double h = beta * (r[0] - r[1]);
     const double tail = log1p(exp(-fabs(h)));
-    loss = (1.0 - eps) * (tail + fmax(-h, 0.0)) + eps * (tail + fmax(h, 0.0));
+    // a side of weight 0 is left out: it may be infinite.  A margin that is no number stays one.
+    loss = (eps < 1.0 ? (1.0 - eps) * (tail + fmax(-h, 0.0)) : 0.0) + (eps > 0.0 ? eps * (tail + fmax(h, 0.0)) : 0.0);
     up[0] = beta * (eps - 1.0 / (1.0 + exp(h)));
     up[1] = -up[0];
   }

@@ -395,6 +395,20 @@ def test_preference_far_margins():
     assert loss.tolist() == [0.0, 4e4] and d.reshape(-1).tolist() == [0.0, 0.0, -1.0, 1.0]
 
 
+@pytest.mark.parametrize("S", [1, 5000])
+def test_preference_of_an_impossible_answer(S):
+    """A token of probability 0 makes the margin infinite: the loss of the side that has weight 0 is left out."""
+    lp = torch.zeros(4, S, device=DEV)
+    lp[:, -1] = torch.tensor([-1.0, -math.inf, -math.inf, -1.0], device=DEV)
+    args = (torch.zeros_like(lp), torch.ones_like(lp, dtype=torch.bool), 0.5)
+    loss, rewards, d = ops.preference_loss(lp, *args)
+    assert loss.tolist() == [0.0, math.inf] and d[:, 0].tolist() == [0.0, 0.0, -0.5, 0.5]
+    assert torch.equal(d, d[:, :1].expand(4, S)) and rewards.tolist() == [-0.5, -math.inf, -math.inf, -0.5]
+    loss, _, d = ops.preference_loss(lp, *args, label_smoothing=1.0)
+    assert loss.tolist() == [math.inf, 0.0] and d[:, 0].tolist() == [0.5, -0.5, 0.0, 0.0]
+    assert ops.preference_loss(lp, *args, label_smoothing=0.25)[0].tolist() == [math.inf, math.inf]
+
+
 # ------------------------------------------------------------------ together
 
 def _preference_step(x, V, t, ref, mask, out):

@@ -239,6 +239,18 @@ def test_preference_gradient_is_the_derivative(form, smoothing):
     assert torch.autograd.gradcheck(Op.apply, (lp,))
 
 
+def test_preference_of_an_impossible_answer():
+    """A token of probability 0 makes the margin infinite: the loss of the side that has weight 0 is left out."""
+    lp = torch.tensor([[-1.0], [-math.inf], [-math.inf], [-1.0]])
+    args = (torch.zeros_like(lp), torch.ones_like(lp, dtype=torch.bool), 0.5)
+    loss, rewards, d = ops.preference_loss(lp, *args)
+    assert loss.tolist() == [0.0, math.inf] and d.reshape(-1).tolist() == [0.0, 0.0, -0.5, 0.5]
+    assert rewards.tolist() == [-0.5, -math.inf, -math.inf, -0.5]
+    loss, _, d = ops.preference_loss(lp, *args, label_smoothing=1.0)
+    assert loss.tolist() == [math.inf, 0.0] and d.reshape(-1).tolist() == [0.5, -0.5, 0.0, 0.0]
+    assert ops.preference_loss(lp, *args, label_smoothing=0.25)[0].tolist() == [math.inf, math.inf]
+
+
 def test_preference_step_from_logits_is_the_derivative():
     """Log probabilities, loss and gradient of the logits together, against autograd of the formula in 64 bits."""
     P, S, V = 2, 6, 11
