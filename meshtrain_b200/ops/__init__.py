@@ -762,12 +762,13 @@ def policy_loss_chunk(logits: torch.Tensor, vocab: int, targets: torch.Tensor, o
     valid = (tg >= 0) & (tg < vocab)
     lpd = lp.double()
     ratio = torch.exp(lpd - old)
+    ratio = torch.where((adv == 0) & (ratio == math.inf), 0.0, ratio)  # A rho = 0, however large rho is
     free, bound = -adv * ratio, -adv * ratio.clamp(1.0 - clip_low, 1.0 + clip_high)
     loss = torch.maximum(free, bound)
     d = torch.where((free >= bound) | free.isnan(), free, 0.0)
     if ref is not None:
         back = ref - lpd
-        loss = loss + kl_coef * (torch.expm1(back) - back)
+        loss = loss + kl_coef * torch.where(back == math.inf, math.inf, torch.expm1(back) - back)
         d = d - kl_coef * torch.expm1(back)
     if w is not None:
         valid = valid & (w != 0)

@@ -133,19 +133,21 @@ struct RowInputs {
 };
 
 // Loss and d loss / d logp of one token.  The exponentials of the ratio and of the KL term are fp32
-// (1e-7 of their value); their arguments are differences taken in fp64.
+// (1e-7 of their value); their arguments are differences taken in fp64.  Of what overflows, A rho is 0 where
+// A is, and exp(d) - d - 1 is infinite.
 __device__ __forceinline__ void policy_terms(const PolicyArgs& a, const RowInputs& in, double logp, bool valid,
                                              float* loss, float* coef) {
   *loss = *coef = 0.f;
   if (!valid || in.w == 0.f) return;
   const float ratio = expf((float)(logp - (double)in.old));
   const float lo = (float)(1.0 - a.clip_low), hi = (float)(1.0 + a.clip_high);
-  const float free_ = -in.adv * ratio, bound = -in.adv * fminf(fmaxf(ratio, lo), hi);
+  const float free_ = in.adv == 0.f && ratio == INFINITY ? 0.f : -in.adv * ratio;
+  const float bound = -in.adv * fminf(fmaxf(ratio, lo), hi);
   float l = fmaxf(free_, bound), d = free_ >= bound ? free_ : 0.f;
   if (isnan(free_)) l = d = free_;
   if (a.ref_logps) {
     const float back = (float)((double)in.ref - logp), e = expm1f(back), kl = (float)a.kl_coef;
-    l += kl * (e - back);
+    l += kl * (e == INFINITY ? e : e - back);
     d -= kl * e;
   }
   *loss = in.w * l;

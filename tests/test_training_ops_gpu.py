@@ -321,6 +321,23 @@ def test_policy_loss_chunk(T, V, dtype):
     assert again[2].data_ptr() == x.data_ptr() and x[:, V:].isnan().all()
 
 
+@pytest.mark.parametrize("V", [9, 2051, 50257])
+def test_policy_loss_at_probabilities_of_zero(V):
+    """An old probability of 0 (or a ratio past the type's range) beside an advantage of 0, and a KL term of a
+    token the policy gives probability 0: the formula's limits 0 and infinity, not NaN."""
+    x = torch.zeros(4, V, device=DEV)
+    x[2, 1] = -math.inf
+    t = torch.ones(4, dtype=torch.int64, device=DEV)
+    lp = -math.log(V)
+    old = torch.tensor([-math.inf, -200.0, 0.0, lp], device=DEV)
+    adv = torch.tensor([0.0, 0.0, 1.0, 1.0], device=DEV)
+    loss, _, d = ops.policy_loss_chunk(x, V, t, old, adv)
+    assert loss[:2].tolist() == [0.0, 0.0] and d[:2].eq(0).all()
+    assert loss[2] == 0 and d[2].eq(0).all() and d[3].isfinite().all() and d[3, 1] < 0
+    loss, lps, d = ops.policy_loss_chunk(x, V, t, old, adv, ref_logps=torch.full_like(old, lp), kl_coef=0.5)
+    assert lps[2] == -math.inf and loss[2] == math.inf and loss[[0, 1, 3]].isfinite().all()
+
+
 def test_policy_without_weights_or_reference():
     x, t = _logits(20, 999, torch.bfloat16)
     old, adv = -7 + _rand(20) * 0.1, _rand(20)

@@ -239,6 +239,23 @@ def test_preference_gradient_is_the_derivative(form, smoothing):
     assert torch.autograd.gradcheck(Op.apply, (lp,))
 
 
+def test_policy_loss_at_probabilities_of_zero():
+    """An old probability of 0 (or a ratio past the type's range) beside an advantage of 0, and a KL term of a
+    token the policy gives probability 0: the formula's limits 0 and infinity, not NaN."""
+    V = 9
+    x = torch.zeros(4, V)
+    x[2, 1] = -math.inf
+    t = torch.ones(4, dtype=torch.int64)
+    lp = -math.log(V)
+    old = torch.tensor([-math.inf, -200.0, 0.0, lp])
+    adv = torch.tensor([0.0, 0.0, 1.0, 1.0])
+    loss, _, d = ops.policy_loss_chunk(x, V, t, old, adv)
+    assert loss[:2].tolist() == [0.0, 0.0] and d[:2].eq(0).all()
+    assert loss[2] == 0 and d[2].eq(0).all() and d[3].isfinite().all() and d[3, 1] < 0
+    loss, lps, d = ops.policy_loss_chunk(x, V, t, old, adv, ref_logps=torch.full_like(old, lp), kl_coef=0.5)
+    assert lps[2] == -math.inf and loss[2] == math.inf and loss[[0, 1, 3]].isfinite().all()
+
+
 def test_preference_of_an_impossible_answer():
     """A token of probability 0 makes the margin infinite: the loss of the side that has weight 0 is left out."""
     lp = torch.tensor([[-1.0], [-math.inf], [-math.inf], [-1.0]])
