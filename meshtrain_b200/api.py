@@ -388,9 +388,9 @@ class PipelineTrainer:
 
     def step(self, step: int, inputs: torch.Tensor | None, targets: torch.Tensor | None,
              timed: bool | str = True, extras: dict[str, torch.Tensor] | None = None) -> StepStats:
-        """One global step (``extras``: the per-token tensors of an ``objective``).  With several ranks a failure anywhere in the pipeline
-        raises here (``PeerFailure`` on the ranks that did not fail) instead of
-        leaving the survivors blocked in NCCL."""
+        """One global step (``extras``: the per-token tensors of an ``objective``).  With
+        several ranks a failure anywhere in the pipeline raises here (``PeerFailure`` on
+        the ranks that did not fail) instead of leaving the survivors blocked in NCCL."""
         if self.watch is not None:
             self.watch.check()
         try:

@@ -95,7 +95,8 @@ class ModelConfig(_Section):
     qk_norm: bool | None = None                    # llama: RMS norm of each query and key head before the rotation
     dropout: float | None = Field(None, ge=0, lt=1)  # embedding output and residual branches
 
-    RULES = (_split_blocks_needs_blocks, _block_options_need_blocks, _heads_divide_hidden, _mlp_sizes, _kv_heads_divide_heads)
+    RULES = (_split_blocks_needs_blocks, _block_options_need_blocks, _heads_divide_hidden, _mlp_sizes,
+             _kv_heads_divide_heads)
 
     def spec_kwargs(self) -> dict:
         """Keyword arguments of the model registry for this model."""

@@ -253,7 +253,7 @@ class PipelineEngine:
         if objective is not None and self.is_last and not self._has_fused_loss:
             raise ValueError("an objective needs a model whose last layer is an LM head")
         self._pass = (0, 0)  # step and microbatch of the forward under way
-        self._rng_layers = sum(1 for i in range(spec.num_layers) if i == 0 or spec.global_layer(i) != spec.global_layer(i - 1))
+        self._rng_layers = len({spec.global_layer(i) for i in range(spec.num_layers)})
         self.failure_check = None  # () -> reason or None: set by a trainer that watches its peers
         # NVTX ranges per action and for the optimizer (MESHTRAIN_NVTX=1), for Nsight timelines
         self.nvtx = os.environ.get("MESHTRAIN_NVTX") == "1"
