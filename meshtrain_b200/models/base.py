@@ -54,7 +54,7 @@ class PipelineLayer(nn.Module):
         recomputed forward.  The engine puts them into ``saved`` from the run's seed, the step, the
         microbatch and the layer; without it a pass draws them from torch's CPU generator."""
         if RNG_KEY not in saved:
-            seed, base = torch.randint(0, 2**62, (2,)).tolist()
+            seed, base = torch.randint(0, 2**62, (2,), device="cpu").tolist()
             saved[RNG_KEY] = (seed, base * RNG_SITES % 2**62)
         seed, offset = saved[RNG_KEY]
         return seed, offset + site

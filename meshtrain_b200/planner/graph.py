@@ -133,7 +133,7 @@ def profile_model(spec, microbatch_size: int) -> list[LayerProfile]:
         if h.is_floating_point():
             h = h.to(spec.dtype)
         for i in range(spec.num_layers):
-            layer = spec._make_layer(i).to(spec.dtype)
+            layer = spec._make_layer(i).to(spec.dtype).eval()  # dropout keeps nothing and has no FLOPs to count
             pcount = sum(p.numel() for p in layer.parameters())
             pbytes = sum(p.numel() * p.element_size() for p in layer.parameters())
             inp = h.detach().requires_grad_(h.is_floating_point())

@@ -359,6 +359,23 @@ def test_config_keys():
             parse_config({"model": bad})
 
 
+@pytest.mark.parametrize("cfg", CFGS, ids=IDS)
+def test_meta_profile_is_that_of_the_model_without_dropout(cfg):
+    from meshtrain_b200.planner.graph import profile_model
+
+    with_drop, without = (profile_model(build_model_spec({**cfg, "dropout": p}), 2) for p in (0.2, 0.0))
+    assert with_drop == without
+
+
+def test_random_numbers_come_from_the_cpu_generator_whatever_the_default_device():
+    layer = build_model_spec(CFGS[0]).build_layer(1)
+    torch.manual_seed(3)
+    want = layer._rng({}, 1)
+    torch.manual_seed(3)
+    with torch.device("meta"):
+        assert layer._rng({}, 1) == want
+
+
 def test_planner_counts_the_normalised_heads():
     from meshtrain_b200.planner.graph import analytic_profile
 
