@@ -508,6 +508,7 @@ def qk_norm_rope(qkv, q_gain, k_gain, seq_len: int, heads: int, kv_heads: int, h
     ``qkv`` [T, >= (heads + kv_heads) * head_dim] holds the query heads, then the key heads (columns
     behind them are not read); row t has position t % seq_len.  Each head is scaled by
     ``(mean(x^2) + eps)^-1/2`` times ``q_gain`` / ``k_gain`` [head_dim] and rotated as ``rope_`` does.
+    The kernels take head dimensions that are multiples of 16 up to 256 and refuse others.
     Returns [T, (heads + kv_heads) * head_dim], in ``out`` when given, which must not overlap ``qkv``:
     that is what the backward needs.
     """
