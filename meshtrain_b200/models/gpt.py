@@ -274,6 +274,8 @@ class LMHead(PipelineLayer):
             c1 = min(T, c0 + chunk_tokens)
             lg = buf[: c1 - c0]
             yc = y[c0:c1]
+            if c0:
+                ops.wait_wgrad(buf.device)  # a deferred weight gradient may still read the last chunk's rows
             if logits is None:
                 self._logits(yc, lg)
             to_gradient(lg, c0, c1)

@@ -272,8 +272,18 @@ def deferred_wgrad(enabled: bool = True, timer=None):
             torch.cuda.current_stream(idx).wait_stream(_WGRAD_STREAMS[idx])
 
 
+def wait_wgrad(device: torch.device) -> None:
+    """The current stream waits for the weight gradients deferred so far on ``device``: called before
+    memory that ``linear_wgrad_`` was given is written again (nothing to wait for outside ``deferred_wgrad``)."""
+    if device.index in (getattr(_WGRAD, "used", None) or ()):
+        torch.cuda.current_stream(device).wait_stream(_WGRAD_STREAMS[device.index])
+
+
 def linear_wgrad_(dy: torch.Tensor, x: torch.Tensor, w_grad: torch.Tensor, b_grad: torch.Tensor | None = None) -> None:
-    """w_grad += dy^T x (fp32 accumulate); b_grad += sum_t dy."""
+    """w_grad += dy^T x (fp32 accumulate); b_grad += sum_t dy.
+
+    Inside ``deferred_wgrad`` dy and x may still be read after the call: freeing them is safe, writing
+    them again needs ``wait_wgrad`` first."""
     if _custom(dy, x) and w_grad.dtype == torch.float32:
         ext = extension()
         dy2, x2 = _mat(dy), _mat(x)

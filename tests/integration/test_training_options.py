@@ -327,6 +327,39 @@ def test_losses_in_chunks_match_one_chunk():
     assert torch.allclose(head.logprobs(x, y), want, atol=1e-5)
 
 
+@pytest.mark.parametrize("name", ["fwd_loss", "fwd_preference_loss", "fwd_policy_loss"])
+def test_chunked_losses_wait_for_deferred_weight_gradients(name, monkeypatch):
+    """The chunks share one logits buffer: with weight gradients run as late as a side stream may run them,
+    each still has to see its own chunk's rows."""
+    torch.manual_seed(0)
+    head = build_model_spec(GPT, seed=2).build_layer(3)
+    x, y = torch.randn(4, 12, 32), torch.randint(0, 61, (4, 12))
+    f32 = lambda: torch.randn(4, 12) - 4  # noqa: E731
+    mask = torch.rand(4, 12) < 0.7
+    kw = {"fwd_loss": {}, "fwd_preference_loss": dict(ref_logps=f32(), mask=mask),
+          "fwd_policy_loss": dict(old_logps=f32(), advantages=f32(), mask=mask)}[name]
+
+    def run():
+        grads = {n: torch.zeros_like(q) for n, q in head.named_parameters()}
+        with torch.no_grad():
+            getattr(head, name)(x, y, {}, grads, torch.zeros(()), 0.5, chunk_tokens=7, **kw)
+        return grads
+
+    want = run()
+    real, late = ops.linear_wgrad_, []
+
+    def drain(device=None):
+        while late:
+            real(*late.pop(0))
+
+    monkeypatch.setattr(ops, "linear_wgrad_", lambda *args: late.append(args))
+    monkeypatch.setattr(ops, "wait_wgrad", drain, raising=False)
+    got = run()
+    drain()
+    for n, r in want.items():
+        assert torch.equal(got[n], r), n
+
+
 def test_objective_refusals():
     spec, eng = _engine(GPT, 1, objective=PreferenceObjective())
     x, y = spec.make_batch(0, 4)

@@ -81,14 +81,17 @@ def test_llama_block_with_head_norms_and_dropout(hidden, H, HK):
         assert _rel_l2(grad, w[name].grad) < 3e-2, name
 
 
-def _step(cfg, objective=None, recompute=None, backend="custom"):
+def _step(cfg, objective=None, recompute=None, backend="custom", deferred=True, chunk_tokens=None, repeats=1):
     from meshtrain_b200.parallel.engine import PipelineEngine
 
     ops.set_backend(backend)
     spec = build_model_spec(cfg, seed=7)
     eng = PipelineEngine(spec, layer_range=(0, spec.num_layers), stage=0, num_stages=1, device="cuda:0",
                          num_microbatches=2, optimizer="sgd", lr=0.0, init_on_device=True, objective=objective,
-                         recompute=set(range(1, spec.num_layers - 1)) if recompute else None)
+                         recompute=set(range(1, spec.num_layers - 1)) if recompute else None,
+                         deferred_wgrad=deferred)
+    if chunk_tokens:
+        eng.layers[-1]._chunk_tokens = lambda T: chunk_tokens
     x, y = spec.make_batch(0, 8)
     y = y.clone()
     extras = None
@@ -102,7 +105,8 @@ def _step(cfg, objective=None, recompute=None, backend="custom"):
         if isinstance(objective, PolicyObjective):
             extras |= {"old_logps": lp + noise(), "advantages": 5 * noise()}
     before = ops.launches()
-    st = eng.train_step(4, x.pin_memory(), y.pin_memory(), extras=extras)
+    for _ in range(repeats):  # lr 0: each repeats the last
+        st = eng.train_step(4, x.pin_memory(), y.pin_memory(), extras=extras)
     torch.cuda.synchronize()
     return float(st.loss) / 2, eng.named_gradients_cpu(), ops.launches() - before
 
@@ -132,3 +136,22 @@ def test_recompute_repeats_the_masks():
     assert again == pytest.approx(loss, rel=1e-3)
     for k, r in grads.items():
         assert _rel_l2(other[k], r) < 2e-2, k
+
+
+@pytest.mark.parametrize("objective", [None, PreferenceObjective(0.3), PolicyObjective(kl_coef=0.1)],
+                         ids=["cross-entropy", "preference", "policy"])
+@pytest.mark.parametrize("cfg", [GPT, LLAMA], ids=["gpt", "llama"])
+def test_chunks_of_logits_with_deferred_weight_gradients(cfg, objective):
+    """Eight chunks per microbatch share a logits buffer that weight gradients on the side stream read."""
+    chunked = dict(chunk_tokens=128, repeats=4)
+    _, want, _ = _step(cfg, objective, deferred=False, **chunked)
+    _, one, _ = _step(cfg, objective, deferred=False)
+    _, got, _ = _step(cfg, objective, **chunked)
+    # The head's: the same GEMMs in the same order; fp32 sums whose order is free (split products, column sums)
+    # differ by a few of their 2^-24 half steps: 1e-5.  Below it, attention's backward sums in any order ahead of
+    # bf16 roundings of 2^-8 each: 2e-2, as for a recomputed forward.  One chunk and eight: GEMMs of other shapes,
+    # whose bf16 logits may round differently, which the clip's border sees as above.
+    clip = 0.095 if isinstance(objective, PolicyObjective) else 0.0
+    for k, r in want.items():
+        assert _rel_l2(got[k], r) < (1e-5 if k.startswith("model.layers.3.") else 2e-2), k
+        assert _rel_l2(one[k], r) < 2e-2 + clip, k
