@@ -258,25 +258,25 @@ class LMHead(PipelineLayer):
         else:
             lg[:, :self.vocab] = ops.linear(yc, self.out.weight, self.out.bias)
 
-    def _chunked_loss(self, x, saved, grads, to_gradient, chunk_tokens=None, normed=None, logits=None) -> None:
+    def _chunked_loss(self, x, saved, grads, to_gradient, chunk_tokens=None, normed=None, buf=None, filled=False) -> None:
         """Logits, their gradient and the layer's backward, a chunk of tokens at a time.
 
         ``to_gradient(lg, c0, c1)`` replaces the logits of rows [c0, c1) by their gradient.  ``normed``: the
-        norm's result where a pass before needed it; ``logits``: all rows' logits where it kept them."""
+        norm's result and ``buf`` the logits buffer of a pass before; ``filled``: it holds all rows' logits."""
         B, S, d = x.shape
         T = B * S
         x2 = x.reshape(T, d)
         y, m, r = self._norm(x2) if normed is None else normed
         chunk_tokens = chunk_tokens or self._chunk_tokens(T)
         dy = torch.empty_like(x2)
-        buf = self._logits_buffer(y, chunk_tokens) if logits is None else logits
+        buf = self._logits_buffer(y, chunk_tokens) if buf is None else buf
         for c0 in range(0, T, chunk_tokens):
             c1 = min(T, c0 + chunk_tokens)
             lg = buf[: c1 - c0]
             yc = y[c0:c1]
             if c0:
                 ops.wait_wgrad(buf.device)  # a deferred weight gradient may still read the last chunk's rows
-            if logits is None:
+            if not filled:
                 self._logits(yc, lg)
             to_gradient(lg, c0, c1)
             dl = lg[:, :self.vocab]
@@ -353,7 +353,7 @@ class LMHead(PipelineLayer):
         def backward(lg, c0, c1):
             ops.token_logprobs_bwd(lg, self.vocab, tg[c0:c1], stats[c0:c1], dlogps[c0:c1], out=lg)
 
-        self._chunked_loss(x, saved, grads, backward, chunk_tokens, normed, buf if T <= chunk_tokens else None)
+        self._chunked_loss(x, saved, grads, backward, chunk_tokens, normed, buf, T <= chunk_tokens)
 
     def forward(self, x):  # autograd path
         if ops.backend() == "torch" or not x.is_cuda:

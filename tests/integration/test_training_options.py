@@ -360,6 +360,21 @@ def test_chunked_losses_wait_for_deferred_weight_gradients(name, monkeypatch):
         assert torch.equal(got[n], r), n
 
 
+@pytest.mark.parametrize("chunk", [48, 7])
+def test_preference_loss_holds_one_buffer_of_logits(chunk, monkeypatch):
+    """What the memory estimate counts: both passes over the logits go through the same buffer."""
+    head = build_model_spec(GPT, seed=2).build_layer(3)
+    made = []
+    real = head._logits_buffer
+    monkeypatch.setattr(head, "_logits_buffer", lambda *a: made.append(1) or real(*a))
+    grads = {n: torch.zeros_like(q) for n, q in head.named_parameters()}
+    with torch.no_grad():
+        head.fwd_preference_loss(torch.randn(4, 12, 32), torch.randint(0, 61, (4, 12)), {}, grads, torch.zeros(()), 1.0,
+                                 ref_logps=-torch.rand(4, 12), mask=torch.ones(4, 12, dtype=torch.bool),
+                                 chunk_tokens=chunk)
+    assert len(made) == 1
+
+
 def test_objective_refusals():
     spec, eng = _engine(GPT, 1, objective=PreferenceObjective())
     x, y = spec.make_batch(0, 4)
