@@ -19,6 +19,7 @@ the device-side engine instead of TCP stage processes.
 
 from __future__ import annotations
 
+import contextlib
 import datetime
 import os
 
@@ -386,34 +387,44 @@ class PipelineTrainer:
     def is_last(self) -> bool:
         return self.stage == self.world - 1
 
+    @contextlib.contextmanager
+    def _watched(self, what: str):
+        """A pass over all stages: a failure of this rank is reported to the others, and one that another
+        rank reported first is raised as ``PeerFailure``."""
+        if self.watch is None:
+            yield
+            return
+        from meshtrain_b200.parallel.watchdog import PeerFailure
+
+        self.watch.check()
+        try:
+            yield
+        except Exception as exc:
+            peer = self.watch.peer_failure()
+            if peer is not None:  # this rank failed because a peer did
+                raise PeerFailure(peer) from exc
+            self.watch.report(f"{what}: {type(exc).__name__}: {exc}")
+            raise
+
     def step(self, step: int, inputs: torch.Tensor | None, targets: torch.Tensor | None,
              timed: bool | str = True, extras: dict[str, torch.Tensor] | None = None) -> StepStats:
         """One global step (``extras``: the per-token tensors of an ``objective``).  With
         several ranks a failure anywhere in the pipeline raises here (``PeerFailure`` on
         the ranks that did not fail) instead of leaving the survivors blocked in NCCL."""
-        if self.watch is not None:
-            self.watch.check()
-        try:
+        with self._watched(f"step {step}"):
             stats = self.engine.train_step(step, inputs if self.is_first else None,
                                            targets if self.is_last else None, timed=timed,
                                            extras=extras if self.is_last else None)
-        except Exception as exc:
-            if self.watch is not None:
-                from meshtrain_b200.parallel.watchdog import PeerFailure
-
-                peer = self.watch.peer_failure()
-                if peer is not None:  # this rank failed because a peer did
-                    raise PeerFailure(peer) from exc
-                self.watch.report(f"step {step}: {type(exc).__name__}: {exc}")
-            raise
         if self.watch is not None:
             self.watch.beat(step)
         return stats
 
     def logprobs(self, inputs: torch.Tensor | None, targets: torch.Tensor | None) -> torch.Tensor | None:
         """Log probabilities [batch, S] of ``targets`` under the current weights (``PipelineEngine.logprobs``);
-        every rank calls it, the last one gets the result."""
-        return self.engine.logprobs(inputs if self.is_first else None, targets if self.is_last else None)
+        every rank calls it, the last one gets the result.  Failures are handled as in ``step``, for which a
+        pass over several ranks waits for its end.  Interleaved chunks (``virtual_stages`` > 1) are refused."""
+        with self._watched("logprobs"):
+            return self.engine.logprobs(inputs if self.is_first else None, targets if self.is_last else None)
 
     def finish_timing(self, stats: list[StepStats]) -> list[StepStats]:
         """Device timing of steps run with ``timed="deferred"`` (waits for them)."""

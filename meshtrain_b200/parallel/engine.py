@@ -570,6 +570,10 @@ class PipelineEngine:
         finally:
             for layer, mode in zip(self.layers, modes):
                 layer.train(mode)
+        if self.cuda and self.failure_check is not None:  # a peer that failed leaves its receives unanswered
+            done = torch.cuda.Event()
+            done.record()
+            self.wait_event(done)
         return torch.cat(out) if self.is_last else None
 
     def finish_timing(self, stats: StepStats) -> StepStats:

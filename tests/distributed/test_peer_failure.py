@@ -57,3 +57,39 @@ def test_failure_of_one_rank_stops_all_ranks(victim):
         assert o["seconds"] < 25, o                # well inside the process-group timeout
     survivors = [o for i, o in enumerate(outcomes) if i != victim]
     assert any(o["error"] == "PeerFailure" and f"rank {victim}" in o["message"] for o in survivors), survivors
+
+
+def _logprobs_until_failure(victim: int):
+    from meshtrain_b200.api import PipelineTrainer
+
+    trainer = PipelineTrainer(GPT, num_microbatches=2, device="cpu", microbatch_size=2, link_probe=False)
+    x, y = trainer.spec.make_batch(0, 4)
+    outcome = {"rank": trainer.rank, "got": trainer.logprobs(x, y) is not None, "errors": []}
+    if trainer.rank == victim:
+        def failing(*args):
+            raise RuntimeError("injected failure before launching the pass")
+        trainer.engine.logprobs = failing
+    t0 = time.monotonic()
+    for call in (lambda: trainer.logprobs(x, y), lambda: trainer.step(0, x, y)):
+        try:
+            call()
+        except Exception as exc:  # noqa: BLE001 - the outcome is what the test checks
+            outcome["errors"].append(f"{type(exc).__name__}: {exc}"[:300])
+    outcome["seconds"] = time.monotonic() - t0
+    if trainer.rank == victim:
+        time.sleep(3)  # keep the store's host up while the others read the report
+    trainer.close()
+    return outcome
+
+
+@pytest.mark.parametrize("victim", [0, 1, 2])
+def test_failure_in_logprobs_stops_all_ranks(victim):
+    results = {r["rank"]: r for r in spawn_ranks(_logprobs_until_failure, 3, victim, timeout_s=120,
+                                                 env={"MESHTRAIN_PG_TIMEOUT_S": "30"})}
+    assert [results[r]["got"] for r in range(3)] == [False, False, True]
+    assert "injected failure" in results[victim]["errors"][0]
+    for rank, r in results.items():
+        assert r["seconds"] < 15, r
+        if rank != victim:  # at the latest the next pass tells: a send may be done before anyone receives it
+            assert r["errors"] and r["errors"][0].startswith("PeerFailure"), r
+            assert f"rank {victim}: logprobs: RuntimeError: injected" in r["errors"][0], r
