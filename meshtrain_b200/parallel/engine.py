@@ -546,6 +546,8 @@ class PipelineEngine:
         batch = inputs if self.is_first else targets if self.is_last else None
         if (self.is_first and inputs is None) or (self.is_last and targets is None):
             raise ValueError("the first stage needs inputs, the last needs targets")
+        if batch is None and self.microbatch_size is None:
+            raise ValueError("a middle stage needs the engine's microbatch_size")
         rows = self.microbatch_size * M if batch is None else batch.shape[0]
         if rows % M:
             raise ValueError("batch size must be divisible by the number of microbatches")

@@ -393,6 +393,15 @@ def test_objective_refusals():
         _engine({"type": "mlp", "dtype": "float32"}, 1, objective=PreferenceObjective())
 
 
+def test_logprobs_of_a_middle_stage_needs_its_batch():
+    from meshtrain_b200.parallel.engine import PipelineEngine
+
+    spec = build_model_spec(GPT, seed=3)
+    middle = PipelineEngine(spec, layer_range=(1, 2), stage=1, num_stages=3, device="cpu", num_microbatches=2)
+    with pytest.raises(ValueError, match="microbatch_size"):
+        middle.logprobs()
+
+
 def test_config_keys():
     model = {k: v for k, v in LLAMA.items()}
     cfg = parse_config({"model": {**model, "qk_norm": True, "dropout": 0.1}})
