@@ -397,7 +397,8 @@ def test_logprobs_of_a_middle_stage_needs_its_batch():
     from meshtrain_b200.parallel.engine import PipelineEngine
 
     spec = build_model_spec(GPT, seed=3)
-    middle = PipelineEngine(spec, layer_range=(1, 2), stage=1, num_stages=3, device="cpu", num_microbatches=2)
+    middle = PipelineEngine(spec, layer_range=(1, 2), stage=1, num_stages=3, device="cpu", num_microbatches=2,
+                            links=object())
     with pytest.raises(ValueError, match="microbatch_size"):
         middle.logprobs()
 
