@@ -372,6 +372,8 @@ class PipelineEngine:
         """
         M = self.M
         dev = self.device
+        if any(t is not None and t.shape[0] % M for t in (inputs, targets)):
+            raise ValueError("batch size must be divisible by the number of microbatches")
         if self.is_first:
             if inputs is None:
                 raise ValueError("the first stage needs inputs")
@@ -392,8 +394,6 @@ class PipelineEngine:
         else:
             raise ValueError("a middle stage needs the engine's microbatch_size")
         mb_size = batch // M
-        if batch % M:
-            raise ValueError("batch size must be divisible by the number of microbatches")
         v = self.chunks
         if v == 1:
             ledger = StepLedger(self.stage, self.num_stages, M, step, self.schedule, self.max_inflight)

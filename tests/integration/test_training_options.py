@@ -403,6 +403,16 @@ def test_logprobs_of_a_middle_stage_needs_its_batch():
         middle.logprobs()
 
 
+@pytest.mark.parametrize("rows", [2, 5])
+def test_a_batch_that_the_microbatches_do_not_divide_is_refused_alike(rows):
+    for objective in (None, PreferenceObjective()):
+        spec, eng = _engine(GPT, 4, objective=objective)
+        x, y = spec.make_batch(0, rows)
+        extras = objective and {"ref_logps": torch.zeros(rows, 12), "mask": torch.ones(rows, 12, dtype=torch.bool)}
+        with pytest.raises(ValueError, match="divisible by the number of microbatches"):
+            eng.train_step(0, x, y, extras=extras)
+
+
 def test_config_keys():
     model = {k: v for k, v in LLAMA.items()}
     cfg = parse_config({"model": {**model, "qk_norm": True, "dropout": 0.1}})
