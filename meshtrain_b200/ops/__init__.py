@@ -540,7 +540,7 @@ def qk_norm_rope_bwd(dqk, qkv, q_gain, k_gain, seq_len: int, heads: int, kv_head
                      dq_gain: torch.Tensor, dk_gain: torch.Tensor, eps: float = 1e-5,
                      out: torch.Tensor | None = None) -> torch.Tensor:
     """Gradient of ``qk_norm_rope``: returns that of ``qkv``'s query and key columns, and adds the gains'
-    to ``dq_gain`` / ``dk_gain`` (fp32 [head_dim]).
+    to ``dq_gain`` / ``dk_gain`` (fp32 [head_dim]; beside fp64 rows, which have no kernel, fp64 too).
 
     ``dqk`` [T, >= (heads + kv_heads) * head_dim] is the gradient of the result.  ``out`` may be ``dqk``
     itself (columns behind the heads stay as they are) or memory that does not overlap the inputs.
@@ -554,8 +554,8 @@ def qk_norm_rope_bwd(dqk, qkv, q_gain, k_gain, seq_len: int, heads: int, kv_head
     _require(dqk.dim() == 2 and dqk.shape[0] == T and dqk.shape[1] >= cols and dqk.dtype == qkv.dtype
              and dqk.device == qkv.device, f"qk_norm_rope_bwd: dqk must be [rows, >= {cols}] of qkv's dtype and device")
     for g, what in ((dq_gain, "dq_gain"), (dk_gain, "dk_gain")):
-        _require(tuple(g.shape) == (head_dim,) and g.dtype == _acc(qkv) and g.device == qkv.device
-                 and g.is_contiguous(), f"qk_norm_rope_bwd: {what} must be contiguous {_acc(qkv)} [head_dim]")
+        _require(tuple(g.shape) == (head_dim,) and g.dtype in (torch.float32, _acc(qkv)) and g.device == qkv.device
+                 and g.is_contiguous(), f"qk_norm_rope_bwd: {what} must be contiguous torch.float32 [head_dim]")
     res = _out_rows("qk_norm_rope_bwd", out, qkv, T, cols)
     dt, half = _acc(qkv), head_dim // 2
     x = qkv[:, :cols].to(dt).reshape(T, -1, head_dim)

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from meshtrain_b200 import ops
+from meshtrain_b200.models.llama import LlamaBlock
 from tests import training_ops_oracle as oracle
 
 
@@ -64,6 +65,22 @@ def test_qk_norm_rope_gradient_is_the_derivative():
             return dx, dg[0], dg[1]
 
     assert torch.autograd.gradcheck(Op.apply, (x, *gains))
+
+
+def test_qk_norm_rope_gains_of_64_bit_rows():
+    """Gradients are held in fp32 whatever the model's type; beside 64-bit rows either type takes them."""
+    T, shape = 5, (3, 2, 1, 6, 100.0)
+    x, dy = (torch.randn(T, 18, dtype=torch.float64) for _ in range(2))
+    gq, gk = (torch.randn(6, dtype=torch.float64) for _ in range(2))
+    wide, narrow = (torch.zeros(2, 6, dtype=dt) for dt in (torch.float64, torch.float32))
+    dx = [ops.qk_norm_rope_bwd(dy, x, gq, gk, *shape, g[0], g[1]) for g in (wide, narrow)]
+    assert torch.equal(*dx)
+    oracle.close(narrow, wide, torch.zeros_like(wide))
+
+    block = LlamaBlock(32, 4, 2, 48, qk_norm=True).double()
+    h = torch.randn(2, 4, 32, dtype=torch.float64, requires_grad=True)
+    block(h).backward(torch.ones_like(h))
+    assert all(p.grad.isfinite().all() and p.grad.any() for p in block.parameters()) and h.grad.dtype == h.dtype
 
 
 @pytest.mark.parametrize("shape", [(1,), (3, 5), (64, 33), (0, 4)])
