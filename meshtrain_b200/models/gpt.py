@@ -183,6 +183,11 @@ class Block(PipelineLayer):
         return super().forward(x)
 
 
+def _at_least(t, dtype):
+    """``t`` widened to ``dtype``, as the losses of a float64 head take their per-token tensors."""
+    return t.to(torch.promote_types(t.dtype, dtype))
+
+
 class LMHead(PipelineLayer):
     """Final LayerNorm + vocabulary projection.
 
@@ -258,7 +263,8 @@ class LMHead(PipelineLayer):
         else:
             lg[:, :self.vocab] = ops.linear(yc, self.out.weight, self.out.bias)
 
-    def _chunked_loss(self, x, saved, grads, to_gradient, chunk_tokens=None, normed=None, buf=None, filled=False) -> None:
+    def _chunked_loss(self, x, saved, grads, to_gradient, chunk_tokens=None, normed=None, buf=None,
+                      filled=False) -> None:
         """Logits, their gradient and the layer's backward, a chunk of tokens at a time.
 
         ``to_gradient(lg, c0, c1)`` replaces the logits of rows [c0, c1) by their gradient.  ``normed``: the
@@ -306,9 +312,10 @@ class LMHead(PipelineLayer):
         """``fwd_loss`` with the clipped policy loss (``ops.policy_loss_chunk``), averaged over the tokens
         that ``mask`` marks; all per-token tensors are [B, S]."""
         T = x.shape[0] * x.shape[1]
-        flat = lambda t: None if t is None else t.reshape(T)  # noqa: E731
-        tg, old, ref, adv = flat(targets), flat(old_logps), flat(ref_logps), flat(advantages)
-        w = flat(mask).to(torch.float32)
+        acc = ops._acc(x)
+        flat = lambda t: None if t is None else _at_least(t.reshape(T), acc)  # noqa: E731
+        tg, old, ref, adv = targets.reshape(T), flat(old_logps), flat(ref_logps), flat(advantages)
+        w = flat(mask).to(acc)
         w = w / w.sum().clamp(min=1.0)
 
         def policy(lg, c0, c1):
@@ -337,7 +344,8 @@ class LMHead(PipelineLayer):
         y = normed[0]
         chunk_tokens = chunk_tokens or self._chunk_tokens(T)
         buf = self._logits_buffer(y, chunk_tokens)
-        acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+        acc = ops._acc(x)
+        ref_logps = _at_least(ref_logps, acc)
         logps = torch.empty(T, device=x.device, dtype=acc)
         stats = torch.empty(T, 2, device=x.device, dtype=acc)
         for c0 in range(0, T, chunk_tokens):

@@ -327,6 +327,37 @@ def test_losses_in_chunks_match_one_chunk():
     assert torch.allclose(head.logprobs(x, y), want, atol=1e-5)
 
 
+@pytest.mark.parametrize("name", ["fwd_preference_loss", "fwd_policy_loss"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_losses_of_a_64_bit_head(name, dtype):
+    """fp32 per-token tensors (what ``logprobs`` and an engine's step bring) or 64-bit ones, which an fp32 head
+    refuses."""
+    torch.manual_seed(0)
+    head = build_model_spec(GPT, seed=2).build_layer(3).double()
+    x, y = torch.randn(4, 12, 32, dtype=torch.float64), torch.randint(0, 61, (4, 12))
+    lp = head.logprobs(x, y).detach()
+    adv = torch.randn(4, 12)
+    kw = dict(ref_logps=lp) if name == "fwd_preference_loss" else dict(old_logps=lp, advantages=adv)
+    kw = {k: v.to(dtype) for k, v in kw.items()} | {"mask": torch.rand(4, 12) < 0.7}
+
+    def run(head, x):
+        grads, loss, saved = {n: torch.zeros(q.shape) for n, q in head.named_parameters()}, torch.zeros(()), {}
+        with torch.no_grad():
+            getattr(head, name)(x, y, saved, grads, loss, 1.0, **kw)
+        return loss, saved["dx"], grads
+
+    loss, dx, grads = run(head, x)
+    assert dx.dtype == torch.float64
+    single = head.float()
+    if dtype == torch.float64:
+        with pytest.raises(ValueError):
+            run(single, x.float())
+        return
+    loss32, dx32, grads32 = run(single, x.float())
+    assert torch.allclose(loss, loss32, rtol=1e-5, atol=1e-6)
+    _same({"dx": dx.float(), **grads}, {"dx": dx32, **grads32}, 1e-4)
+
+
 @pytest.mark.parametrize("name", ["fwd_loss", "fwd_preference_loss", "fwd_policy_loss"])
 def test_chunked_losses_wait_for_deferred_weight_gradients(name, monkeypatch):
     """The chunks share one logits buffer: with weight gradients run as late as a side stream may run them,
