@@ -540,7 +540,7 @@ def qk_norm_rope_bwd(dqk, qkv, q_gain, k_gain, seq_len: int, heads: int, kv_head
                      dq_gain: torch.Tensor, dk_gain: torch.Tensor, eps: float = 1e-5,
                      out: torch.Tensor | None = None) -> torch.Tensor:
     """Gradient of ``qk_norm_rope``: returns that of ``qkv``'s query and key columns, and adds the gains'
-    to ``dq_gain`` / ``dk_gain`` (fp32 [head_dim]; beside fp64 rows, which have no kernel, fp64 too).
+    to ``dq_gain`` / ``dk_gain`` (fp32 [head_dim]; beside fp64 rows, which have no kernel, fp64 too), which may be one tensor.
 
     ``dqk`` [T, >= (heads + kv_heads) * head_dim] is the gradient of the result.  ``out`` may be ``dqk``
     itself (columns behind the heads stay as they are) or memory that does not overlap the inputs.

@@ -365,10 +365,16 @@ Tensor qk_norm_rope_bwd(const Tensor& dqk, const Tensor& qkv, const Tensor& gq, 
                           g->device() == qkv.device() && g->is_contiguous(),
                       "qk_norm_rope_bwd: dq_gain and dk_gain must be contiguous float32 [head_dim]");
   if (in.a.rows == 0) return in.out;
+  // One gradient for both gains (or two that share memory): the kernel adds to either without order, so the
+  // key gain's sum is formed beside it and added after.
+  const auto *q0 = dgq.data_ptr<float>(), *k0 = dgk.data_ptr<float>();
+  const bool shared = q0 < k0 + hd && k0 < q0 + hd;
+  Tensor dk = shared ? torch::zeros({hd}, dgk.options()) : dgk;
   auto partial = torch::empty({mt::qk_norm_rope_blocks(in.a.rows, in.a.H + in.a.HK, in.a.hd), 2 * hd}, dgq.options());
   MT_CHECK_LAUNCH(mt::qk_norm_rope_bwd(in.a, dy.data_ptr(), dy.stride(0), partial.data_ptr<float>(),
-                                       dgq.data_ptr<float>(), dgk.data_ptr<float>(), stream_of(qkv)),
+                                       dgq.data_ptr<float>(), dk.data_ptr<float>(), stream_of(qkv)),
                   "qk_norm_rope_bwd");
+  if (shared) dgk.add_(dk);
   return in.out;
 }
 

@@ -125,6 +125,22 @@ def test_qk_norm_rope_past_2_to_the_31_elements():
     assert dy[:-3, :(H + HK) * hd].count_nonzero() == 0
 
 
+def test_qk_norm_rope_one_gradient_for_both_gains():
+    """A gain that query and key heads share has one gradient buffer; buffers may also overlap in part."""
+    T, seq, H, HK, hd = 400, 50, 5, 2, 64
+    x, dy, g = _rand(T, (H + HK) * hd), _rand(T, (H + HK) * hd), _rand(hd)
+    shape = (seq, H, HK, hd, 10000.0)
+    dq, dk = torch.zeros(2, hd, device=DEV)
+    dx = ops.qk_norm_rope_bwd(dy, x, g, g, *shape, dq, dk)
+    for shift in (0, 8, hd - 1, hd):
+        both = torch.zeros(2 * hd, device=DEV)
+        got = ops.qk_norm_rope_bwd(dy, x, g, g, *shape, both[:hd], both[shift:shift + hd])
+        want = torch.zeros_like(both)
+        want[:hd] += dq
+        want[shift:shift + hd] += dk
+        assert torch.equal(got, dx) and torch.equal(both, want)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_qk_norm_rope_layouts(dtype):
     """Rows on no 16-byte boundary, a wide row stride, a transposed layout and gains inside a larger buffer."""

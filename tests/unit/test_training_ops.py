@@ -83,6 +83,14 @@ def test_qk_norm_rope_gains_of_64_bit_rows():
     assert all(p.grad.isfinite().all() and p.grad.any() for p in block.parameters()) and h.grad.dtype == h.dtype
 
 
+def test_qk_norm_rope_one_gradient_for_both_gains():
+    x, dy, g = torch.randn(5, 18), torch.randn(5, 18), torch.randn(6)
+    apart, shared = torch.zeros(2, 6), torch.zeros(6)
+    ops.qk_norm_rope_bwd(dy, x, g, g, 3, 2, 1, 6, 100.0, apart[0], apart[1])
+    ops.qk_norm_rope_bwd(dy, x, g, g, 3, 2, 1, 6, 100.0, shared, shared)
+    assert torch.equal(shared, apart.sum(0))
+
+
 @pytest.mark.parametrize("shape", [(1,), (3, 5), (64, 33), (0, 4)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_dropout(shape, dtype):
