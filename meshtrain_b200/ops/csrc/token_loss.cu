@@ -261,9 +261,13 @@ struct RowGrad {
   __device__ __forceinline__ RowGrad(Stat st, float c, int t)
       : z(finite_or_zero(st.m)), f(-c / st.s), coef(c), target(t) {}
 
-  __device__ __forceinline__ float one(float x, int c) const {
-    return coef == 0.f ? 0.f : fmaf(exp_diff(x, z), f, c == target ? coef : 0.f);
+  // The target's own entry; s is the row's sum.  Beside an infinite coefficient (a ratio past the type's range, a
+  // KL term at probability 0) the two parts would be infinities of either sign, so it is multiplied out there.
+  __device__ __forceinline__ float at_target(float x, float s) const {
+    const float e = exp_diff(x, z);
+    return isinf(coef) ? coef * (1.f - e / s) : fmaf(e, f, coef);
   }
+  __device__ __forceinline__ float elsewhere(float x) const { return coef == 0.f ? 0.f : exp_diff(x, z) * f; }
   // The gradient of a vector that does not hold the target.  16-bit results are rounded to 11 bits or
   // fewer, so the low part of log2(e), which changes 1e-8 |x - m| of them, is left out there.
   template <class T>
@@ -285,9 +289,9 @@ struct RowGrad {
     }
     pack8(g, r);
   }
-  // The gradient of any vector, at column c; zeros in a masked row, whatever it holds.
+  // The gradient of any vector, at column c, with the target's entry given; zeros in a masked row, whatever it holds.
   template <class T>
-  __device__ __forceinline__ void vector(const Log2e& l, Raw8<T>& r, int c) const {
+  __device__ __forceinline__ void vector(const Log2e& l, Raw8<T>& r, int c, float entry) const {
     if (coef == 0.f) {
 #pragma unroll
       for (int q = 0; q < (int)sizeof(Raw8<T>) / 16; ++q) r.q[q] = make_uint4(0, 0, 0, 0);
@@ -295,7 +299,7 @@ struct RowGrad {
       float g[8];
       unpack8(r, g);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] = one(g[j], c + j);
+      for (int j = 0; j < 8; ++j) g[j] = c + j == target ? entry : elsewhere(g[j]);
       pack8(g, r);
     } else {
       plain(l, r);
@@ -311,7 +315,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32, WARPS == 1 ? 4 
   constexpr int BLOCK = WARPS == 1 ? 256 : TEAM;
   extern __shared__ uint4 stage_mem[];
   __shared__ float2 pairs[2][WARPS * CL];  // of all the cluster's warps, for even and odd turns
-  __shared__ float sh_coef;
+  __shared__ float sh_coef, sh_entry;
   __shared__ int sh_target;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tid = WARPS == 1 ? lane : threadIdx.x;  // within the block's share of the team
@@ -430,6 +434,7 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32, WARPS == 1 ? 4 
         if (lane == 0) {
           sh_coef = c;
           sh_target = (int)in.t;  // only looked at when it is one: otherwise the coefficient is 0
+          if (POLICY) sh_entry = RowGrad(st, c, sh_target).at_target(in.xt, st.s);
         }
       }
       if (POLICY) {
@@ -439,12 +444,13 @@ __global__ void __launch_bounds__(WARPS == 1 ? 256 : WARPS * 32, WARPS == 1 ? 4 
     }
     if (POLICY) {
       const RowGrad grad(st, coef, (WARPS == 1 ? (int)in.t : sh_target) - c0);
+      const float entry = WARPS == 1 ? grad.at_target(in.xt, st.s) : sh_entry;
       T* out = (T*)a.p.out + row * a.p.ldo + c0;
 #pragma unroll
       for (int k = 0; k < kVecs; ++k) {
         const int c = (k * TEAM + tid) * 8;
         if (c < cols) {
-          grad.vector(log2e, raw[k], c);
+          grad.vector(log2e, raw[k], c, entry);
           if (c + 8 <= cols) {
             straw8(out + c, raw[k]);
           } else {
@@ -587,7 +593,7 @@ __global__ void __launch_bounds__(NT, policy_blocks(NT)) stream_policy_kernel(Ro
   constexpr int W = NT / 32, NV = sizeof(T) == 2 ? 2 : 1, ROUND = NV * NT, Q = sizeof(Raw8<T>) / 16;
   __shared__ float2 pairs[2][W];
   __shared__ RowInputs coming;  // of the next row, by asynchronous copies (but for the target's logit)
-  __shared__ float sh_coef, sh_xt;
+  __shared__ float sh_coef, sh_entry;
   __shared__ int sh_target;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int V = a.p.V, full = V / 8;
@@ -671,12 +677,12 @@ __global__ void __launch_bounds__(NT, policy_blocks(NT)) stream_policy_kernel(Ro
       if (lane == 0) {
         sh_coef = c;
         sh_target = (int)in.t;  // only looked at when it is one: otherwise the coefficient is 0
-        sh_xt = in.xt;
+        sh_entry = RowGrad(st, c, sh_target).at_target(in.xt, st.s);
       }
     }
     __syncthreads();
     const RowGrad grad(st, sh_coef, sh_target);
-    const float xt = sh_xt;
+    const float entry = sh_entry;
     const bool more = next < a.rows;
     if (more && tid == 0) fetch_inputs(next);
     const T* xn = (const T*)a.p.logits + next * ld + tid * 8;
@@ -738,9 +744,9 @@ __global__ void __launch_bounds__(NT, policy_blocks(NT)) stream_policy_kernel(Ro
       // the target's own entry, by the thread that wrote its vector
       const int tv = grad.target >> 3;
       if (tv < full && tid == (tv < cached ? tv % NT : (tv - cached) % NT))
-        out[grad.target] = from_f32<T>(grad.one(xt, grad.target));
+        out[grad.target] = from_f32<T>(entry);
     }
-    if (tail < V) out[tail] = from_f32<T>(grad.one(xtail, tail));
+    if (tail < V) out[tail] = from_f32<T>(tail == grad.target && grad.coef != 0.f ? entry : grad.elsewhere(xtail));
     copy_async_wait();
     if (more) {
       for (int r = max(0, whole - kLag); r < whole; ++r) add_round(st, mine + r * ROUND * 16);
@@ -791,17 +797,20 @@ __global__ void __launch_bounds__(kGradThreads)
     const int from = (grad.target >> 3) - v0;
     const bool owner = grad.target < full * 8 && from >= 0 && from < kGradVecs * threads_per_row &&
                        from % threads_per_row == 0;
-    const float xt = owner ? to_f32(x[grad.target]) : 0.f;
+    const float entry = owner ? grad.at_target(to_f32(x[grad.target]), st.s) : 0.f;
 #pragma unroll
     for (int k = 0; k < kGradVecs; ++k)
       if (k * threads_per_row < left) {
         grad.plain(log2e, raw[k]);
         straw8(o + (long)(v0 + k * threads_per_row) * 8, raw[k]);
       }
-    if (owner) o[grad.target] = from_f32<T>(grad.one(xt, grad.target));
+    if (owner) o[grad.target] = from_f32<T>(entry);
   }
   if (part == blocks_per_row - 1)
-    for (int c = full * 8 + tid; c < V; c += threads_per_row) o[c] = from_f32<T>(grad.one(to_f32(x[c]), c));
+    for (int c = full * 8 + tid; c < V; c += threads_per_row) {
+      const float xc = to_f32(x[c]);
+      o[c] = from_f32<T>(c == grad.target && grad.coef != 0.f ? grad.at_target(xc, st.s) : grad.elsewhere(xc));
+    }
 }
 
 // A pair of answers (rows 2i: preferred, 2i + 1: rejected) per block, or per cluster of CL blocks that

@@ -527,3 +527,29 @@ def test_qk_norm_rope_captured_twice():
     for _, res in graphs:
         for a, b in zip(res, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,V", LOGITS)
+def test_gradients_of_infinite_coefficients(T, V, dtype):
+    """An upstream gradient past the type's range, and a KL term beside a target of probability 0: every entry is
+    (onehot - softmax) times the infinity, the target's own too, wherever in its row it lies."""
+    x, t = _logits(T, V, dtype)
+    up = torch.full((T,), math.inf, device=DEV)
+    up[1::2] = -math.inf
+    up[::5] = 0.0
+    ref = oracle.dlogits(x, V, t, up)[0]
+    lp, stats = ops.token_logprobs(x, V, t)
+    oracle.close(ops.token_logprobs_bwd(x, V, t, stats, up), ref, torch.zeros_like(ref), "dlogits")
+    # A < 0 and an old probability of 0: rho and the coefficient are +inf
+    zero = torch.zeros(T, device=DEV)
+    _, _, d = ops.policy_loss_chunk(x, V, t, zero - math.inf, zero - 1, (up != 0).float())
+    ref = oracle.dlogits(x, V, t, up.abs())[0]
+    oracle.close(d, ref, torch.zeros_like(ref), "policy")
+    # the KL term of a target of probability 0: -inf for it
+    x[torch.arange(T, device=DEV), t] = -math.inf
+    _, lp, d = ops.policy_loss_chunk(x, V, t, zero, zero, ref_logps=zero - 1, kl_coef=0.1)
+    ref = oracle.dlogits(x, V, t, zero - math.inf)[0]
+    oracle.close(d, ref, torch.zeros_like(ref), "KL term")
+    if V > 1:
+        assert lp.eq(-math.inf).all() and d[torch.arange(T, device=DEV), t].eq(-math.inf).all()

@@ -281,6 +281,19 @@ def test_policy_loss_at_probabilities_of_zero():
     assert lps[2] == -math.inf and loss[2] == math.inf and loss[[0, 1, 3]].isfinite().all()
 
 
+def test_gradients_of_infinite_coefficients():
+    """The target's entry too is (onehot - softmax) times the infinity."""
+    x, t = _logits(3, 7, torch.float32)
+    up = torch.tensor([math.inf, -math.inf, 0.0])
+    lp, stats = ops.token_logprobs(x, 7, t)
+    ref = oracle.dlogits(x, 7, t, up)[0]
+    oracle.close(ops.token_logprobs_bwd(x, 7, t, stats, up), ref, torch.zeros_like(ref))
+    x[torch.arange(3), t] = -math.inf
+    zero = torch.zeros(3)
+    _, _, d = ops.policy_loss_chunk(x, 7, t, zero, zero, ref_logps=zero - 1, kl_coef=0.1)
+    assert d[torch.arange(3), t].eq(-math.inf).all() and d.isinf().all()
+
+
 def test_preference_of_an_impossible_answer():
     """A token of probability 0 makes the margin infinite: the loss of the side that has weight 0 is left out."""
     lp = torch.tensor([[-1.0], [-math.inf], [-math.inf], [-1.0]])
