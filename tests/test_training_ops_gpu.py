@@ -2,6 +2,7 @@
 
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -200,6 +201,27 @@ def test_dropout_layouts_and_garbage():
     y = ops.dropout(bad, 0.5, 1, 2, residual=torch.ones(4000, device=DEV))
     keep = oracle.dropout(bad, 0.5, 1, 2)[2].to(DEV)
     assert y[~keep].eq(1).all() and y[keep].isnan().all()
+
+
+def test_dropout_across_the_high_word_of_the_counter():
+    """Groups 2^32 and on (elements 2^35 and on) count in the counter's second word."""
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("needs 69 GB of device memory")
+    n = (1 << 35) + 4099
+    x = torch.ones(n, dtype=torch.bfloat16, device=DEV)
+    ops.dropout(x, 0.5, 3, 4, out=x)
+    lo, low, half = (1 << 35) - 4096, np.uint64(0xFFFFFFFF), np.uint64(32)
+    g = np.arange(lo // 8, (n + 7) // 8, dtype=np.uint64)
+    assert g[0] >> half == 0 and g[-1] >> half == 1
+    c, k = [g & low, g >> half, np.full_like(g, 4), np.zeros_like(g)], [3, 0]
+    for _ in range(10):
+        a, b = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
+        c = [(b >> half) ^ c[1] ^ np.uint64(k[0]), b & low, (a >> half) ^ c[3] ^ np.uint64(k[1]), a & low]
+        k = [(k[0] + 0x9E3779B9) % 2 ** 32, (k[1] + 0xBB67AE85) % 2 ** 32]
+    bits = np.stack([w.astype("<u4") for w in c], 1).view("<u2").reshape(-1)[:n - lo]
+    assert torch.equal(x[lo:].cpu() != 0, torch.from_numpy(bits >= 32768))
+    del x
+    torch.cuda.empty_cache()
 
 
 def test_dropout_more_than_2_to_the_32_elements():

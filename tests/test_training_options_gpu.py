@@ -130,6 +130,20 @@ def test_engine_on_the_kernels_matches_torch(cfg, objective):
         assert _rel_l2(grads[k], r) < bound, k
 
 
+def test_logprobs_under_a_failure_watch():
+    """With peers to watch, the pass waits for its end on the host, by polling."""
+    from meshtrain_b200.parallel.engine import PipelineEngine
+
+    spec = build_model_spec(LLAMA, seed=7)
+    eng = PipelineEngine(spec, layer_range=(0, spec.num_layers), stage=0, num_stages=1, device="cuda:0",
+                         num_microbatches=2, init_on_device=True)
+    x, y = spec.make_batch(0, 4)
+    want = eng.logprobs(x, y)
+    eng.failure_check = lambda: None
+    got = eng.logprobs(x, y)
+    assert torch.cuda.current_stream().query() and torch.equal(got, want)
+
+
 def test_recompute_repeats_the_masks():
     loss, grads, _ = _step(LLAMA)
     again, other, _ = _step(LLAMA, recompute=True)
