@@ -92,7 +92,9 @@ class ModelConfig(_Section):
     rope_theta: float | None = Field(None, gt=0)
     init_std: float | None = Field(None, gt=0)
     split_blocks: bool = False                     # partition units of half a block (attention / MLP)
-    qk_norm: bool | None = None                    # llama: RMS norm of each query and key head before the rotation
+    # llama: RMS norm of each query and key head before the rotation (on GPUs head dimensions that are multiples
+    # of 16 up to 256; the first forward refuses others)
+    qk_norm: bool | None = None
     dropout: float | None = Field(None, ge=0, lt=1)  # embedding output and residual branches
 
     RULES = (_split_blocks_needs_blocks, _block_options_need_blocks, _heads_divide_hidden, _mlp_sizes,

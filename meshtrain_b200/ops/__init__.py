@@ -175,8 +175,6 @@ def _mat(x: torch.Tensor) -> torch.Tensor:
     return buf[:, :cols]
 
 
-
-
 # ----------------------------------------------------------------------------- linear
 
 def linear(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None = None, *, gelu: bool = False,
@@ -520,7 +518,9 @@ def qk_norm_rope(qkv, q_gain, k_gain, seq_len: int, heads: int, kv_heads: int, h
     ``(mean(x^2) + eps)^-1/2`` times ``q_gain`` / ``k_gain`` [head_dim] and rotated as ``rope_`` does.
     The kernels take head dimensions that are multiples of 16 up to 256 and refuse others.
     Returns [T, (heads + kv_heads) * head_dim], in ``out`` when given, which must not overlap ``qkv``:
-    that is what the backward needs.
+    that is what the backward needs.  On CUDA an ``out`` has its rows on 16-byte boundaries, with a leading
+    dimension that is a multiple of 8 (so in the losses below); inputs of any layout are taken, copied first
+    where their rows are not so.
     """
     if _custom_float(qkv):
         return _EXT.qk_norm_rope_fwd(qkv, q_gain, k_gain, seq_len, heads, kv_heads, head_dim, theta, eps, out)
@@ -614,7 +614,8 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset, residual: torch.Tensor
     is taken to the nearest 1/65536, and the scale is the inverse of that exact keep probability.
     ``seed`` and ``offset`` are 64-bit: one seed per run, another offset for every use of it.  ``offset``
     may be a one-element int64 tensor on x's device, read when the kernel runs, so that a captured graph
-    draws another mask at each replay.  ``out`` may be ``x`` or ``residual``.  Dropped elements add
+    draws another mask at each replay.  ``out`` may be ``x`` or ``residual``; it is contiguous, and on CUDA starts on
+    a 16-byte boundary.  Dropped elements add
     exactly 0, whatever ``x`` holds there.
     """
     cut = round(p * 65536) if 0.0 <= p < 1.0 else 65536
@@ -726,8 +727,9 @@ def token_logprobs_bwd(logits: torch.Tensor, vocab: int, targets: torch.Tensor, 
     ``stats`` is what ``token_logprobs`` returned for these logits.
 
     Rows without a token, rows whose ``dlogps`` is 0 and rows of nothing but -inf get zeros whatever they
-    hold.  ``out`` may be ``logits`` (overwritten); otherwise a new matrix, whose rows are padded
-    to a multiple of 8 columns as the LM head's GEMMs take them.  Returns its first ``vocab`` columns.
+    hold.  ``out`` may be ``logits`` (overwritten; on CUDA only rows as ``qk_norm_rope`` writes them);
+    otherwise a new matrix, whose rows are padded to a multiple of 8 columns as the LM head's GEMMs take
+    them.  Returns its first ``vocab`` columns.
     """
     if _custom_float(logits):
         return _EXT.token_logprobs_bwd(logits, vocab, targets, stats, dlogps, out)

@@ -10,8 +10,8 @@
 //   y = residual + keep x scale      (one rounding; a dropped element adds exactly 0)
 //
 // Bound: DRAM (two or three accesses per element).  16384 x 4096 bf16, forward with residual and
-// gradient: 106 us together, 6.3 TB/s (96% of the copy rate).  Per eight elements the random words take
-// about 80 instructions; four groups' loads per thread are in flight meanwhile.
+// gradient: 106 us together, 6.3 TB/s (96% of the copy rate).  Eight elements' random words are ten rounds
+// of two 32-bit products and four exclusive-ors; four groups' loads per thread are in flight meanwhile.
 #include <cuda_runtime.h>
 
 #include "mt_api.h"
@@ -39,7 +39,7 @@ __device__ __forceinline__ uint4 philox4x32(uint4 c, const RoundKeys& keys) {
 }
 
 // N groups of eight elements per thread, kThreads groups apart; all loads are issued ahead of the
-// random words, which take about 90 instructions a group.
+// random words, which are most of a group's instructions.
 template <class T, bool RESIDUAL, int N>
 __global__ void __launch_bounds__(kThreads)
     dropout_kernel(const T* x, const T* residual, T* y, long n, uint32_t cut, float scale, uint64_t offset,

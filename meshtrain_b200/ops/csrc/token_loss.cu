@@ -6,7 +6,8 @@
 // logit of the type's lowest value a log-sum-exp could not hold log s.  A target outside [0, V) marks
 // a row without a token: logp 0, gradient 0.  Logits of -inf have probability 0; a row of nothing but
 // -inf has m = logp = -inf, s = 0 and gradient 0.  NaN and +inf propagate within their row, unless the
-// row's weight (or upstream gradient) is 0: such a row's gradient is 0 whatever it holds.
+// row's weight (or upstream gradient) is 0: such a row's gradient is 0 whatever it holds.  An infinite
+// coefficient makes every entry ([c = t] - p_c) times that infinity.
 //
 // Sums are fp32; logp is formed in fp64 from the fp32 maximum and sum, so that it carries one rounding.
 // Exponentials are ex2 of (x - m) log2(e) with the constant in two parts: with one fp32 constant every
