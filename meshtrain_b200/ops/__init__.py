@@ -614,9 +614,8 @@ def dropout(x: torch.Tensor, p: float, seed: int, offset, residual: torch.Tensor
     is taken to the nearest 1/65536, and the scale is the inverse of that exact keep probability.
     ``seed`` and ``offset`` are 64-bit: one seed per run, another offset for every use of it.  ``offset``
     may be a one-element int64 tensor on x's device, read when the kernel runs, so that a captured graph
-    draws another mask at each replay.  ``out`` may be ``x`` or ``residual``; it is contiguous, and on CUDA starts on
-    a 16-byte boundary.  Dropped elements add
-    exactly 0, whatever ``x`` holds there.
+    draws another mask at each replay.  ``out`` may be ``x`` or ``residual``; it is contiguous, and on
+    CUDA starts on a 16-byte boundary.  Dropped elements add exactly 0, whatever ``x`` holds there.
     """
     cut = round(p * 65536) if 0.0 <= p < 1.0 else 65536
     _require(cut < 65536, f"dropout: p must be in [0, 1) and round below 1, got {p}")
